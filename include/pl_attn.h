@@ -57,6 +57,61 @@ extern "C" {
 #define PL_SPLIT_SEQS 0       /* pl_attn_init_devices: slots spread over devices */
 #define PL_SPLIT_KV   1       /* pl_attn_init_devices: every slot's rows spread  */
 
+/* ---- Rotations and the 8-bit cache: their constants and plain structs
+ *      (the calls are described further down) ---- */
+
+/* element types of activations */
+#define PL_F32  0
+#define PL_F16  1
+#define PL_BF16 2
+
+/* frequency scaling; f_i = base^(-2i/dim) is the frequency of pair i */
+#define PL_ROPE_SCALE_NONE   0
+#define PL_ROPE_SCALE_LINEAR 1  /* f_i / factor */
+#define PL_ROPE_SCALE_YARN   2  /* ramp from f_i (pairs that turn more than `high`
+                                 * times in orig_len positions) to f_i / factor
+                                 * (fewer than `low`); cosine and sine times
+                                 * 0.1 ln(factor) + 1 */
+#define PL_ROPE_SCALE_LLAMA3 3  /* f_i above `high` turns in orig_len, f_i / factor
+                                 * below `low`, mixed linearly in the turns between */
+#define PL_ROPE_MAX_PAIRS 128
+
+/* A rotation, filled by pl_rope_init and read by every call that takes it;
+ * plain data, may be copied. */
+typedef struct {
+    int type;       /* PL_ROPE_LLAMA or PL_ROPE_QWEN */
+    int head_dim;   /* elements of a head */
+    int dim;        /* rotated elements, the first of the head; 0: none */
+    int reserved;
+    double gain;    /* factor on cosine and sine */
+    double half_turns[PL_ROPE_MAX_PAIRS];  /* f_i / pi */
+} pl_rope;
+
+#define PL_KV8_INT8 0   /* code in -127..127, scale = max |x| / 127            */
+#define PL_KV8_E4M3 1   /* code an e4m3 float (no NaN), scale = max |x| / 448  */
+#define PL_KV8_PAGE  64
+#define PL_KV8_BLOCK 16
+
+typedef struct {
+    int device;
+    int n_layers, n_heads, n_kv_heads, head_dim;  /* head_dim 64 or 128; n_heads /
+                                                   * n_kv_heads 1..8, any integer */
+    int n_pages;    /* pages of the pool */
+    int n_seqs;     /* sequence slots */
+    int max_pages;  /* pages of a slot, at most */
+    int format;     /* PL_KV8_INT8 or PL_KV8_E4M3 */
+    int owned;      /* set by pl_kv8_alloc */
+    pl_rope rope;   /* applied to q and k (dim 0: they come rotated) */
+    /* device memory, 256-byte aligned (books: 4-byte): */
+    void  *codes;   /* [n_pages][n_layers][n_kv_heads][2][64][head_dim] bytes */
+    float *scales;  /* [n_pages][n_layers][n_kv_heads][2][4] */
+    int   *table;   /* [n_seqs][max_pages], -1 where there is none */
+    int   *lens;    /* [n_seqs] */
+    int   *refs;    /* [n_pages] */
+    void  *work;    /* pl_kv8_work_bytes, zero before the first call */
+    size_t work_bytes;
+} pl_kv8;
+
 #ifndef PL_ATTN_DISABLED
 
 /* ---- Lifecycle (cf. gpu_init / gpu_available / gpu_shutdown,
@@ -349,6 +404,137 @@ int  pl_attn_block_prefill_dev(int seq, int layer, int start_pos, int n_tok,
  * [n][dim] (Wo: [n][n_heads*head_dim]), y [n][rows of W].  No RMSNorm. */
 int  pl_attn_proj(int layer, int which, int n, const float *x, float *y);
 
+/* ---- Rotary positions as an operator of their own ----
+ *
+ * The calls above rotate whole heads by the host's tables.  These rotate
+ * rows in device memory: both layouts of rope() (tensor.c:533-603), part of
+ * the head, frequencies scaled for long contexts, FP32 / FP16 / BF16, and
+ * the adjoint of the rotation (its gradient).  They and the calls on the
+ * 8-bit cache below need no module context; the current device is used. */
+
+/* head_dim a multiple of 8, 8..256; dim even, 0..head_dim (Qwen pairs i with
+ * i + dim/2).  factor, orig_len, low and high as the scaling needs them.
+ * Needs no device. */
+int  pl_rope_init(pl_rope *r, int type, int head_dim, int dim, double base,
+                  int scaling, double factor, int orig_len, double low,
+                  double high);
+
+/* Rotate n rows: row i holds n_heads heads of q at d_q + i*q_stride and
+ * n_kv_heads of k at d_k + i*k_stride (elements of `dtype`; either head count
+ * may be 0), written to the _out rows, which may be the same memory (in
+ * place) but must not overlap otherwise.  Row i is at position d_pos[i] >= 0.
+ * adjoint != 0 applies the transpose: the gradient with respect to the input
+ * from the gradient with respect to the output.  Any stride and alignment;
+ * 16-byte aligned rows and a dim that is a multiple of 16 are fastest.
+ * Asynchronous on `stream`; may be captured. */
+int  pl_rope_rows_dev(const pl_rope *r, int dtype, int n, const int *d_pos,
+                      int n_heads, const void *d_q, long long q_stride,
+                      void *d_q_out, long long q_out_stride, int n_kv_heads,
+                      const void *d_k, long long k_stride, void *d_k_out,
+                      long long k_out_stride, int adjoint, void *stream);
+
+/* ---- The 8-bit paged KV cache ----
+ *
+ * A second cache for engines that keep activations on the device: half the
+ * bytes of the FP16 cache, held in pages that sequences share.  A page holds
+ * PL_KV8_PAGE rows of every layer; K and V are 8-bit codes with one FP32
+ * scale for each block of PL_KV8_BLOCK rows and KV head, value = code *
+ * scale.  A sequence slot has `lens[slot]` rows in the pages
+ * table[slot][0 ..]; refs[page] counts the sequences that hold a page (0:
+ * free).  All of it is plain device memory, laid out as written below and
+ * open to the engine; every book is changed on the device, in stream order,
+ * so that a whole step can be captured in a CUDA graph.
+ *
+ * A step: pl_kv8_resize_dev grows the sequences by their new tokens, then
+ * per layer pl_kv8_decode_dev (one token each) or pl_kv8_append_dev and
+ * pl_kv8_attend_dev (several) run over it.
+ *
+ * No counterpart in the reference, whose cache is FP16 and belongs to one
+ * sequence (model.c:612-619).
+ *
+ * One stream at a time per cache: its calls share the workspace, so calls
+ * that could overlap on the GPU (two streams, two captured graphs) must be
+ * ordered by the caller.  Different caches are independent.  The current
+ * device must be the cache's (PL_EDEVICE).  Arrays of a call are device
+ * memory; a slot, row count or page out of range that a kernel finds there
+ * leaves its entry (its call, for the page operations) undone and is
+ * reported by pl_kv8_status as PL_EARG.  Slots of one call are distinct.
+ * Inputs and outputs are `dtype` rows of heads x head_dim elements, 16-byte
+ * aligned with strides (in elements) that are multiples of 16 bytes. */
+/* Bytes of the workspace of a cache of this shape. */
+int  pl_kv8_work_bytes(const pl_kv8 *c, size_t *bytes);
+
+/* Allocate every array of c (whose shape is filled in) on c->device, empty,
+ * and free them again.  An engine with a pool of its own fills in the
+ * pointers instead. */
+int  pl_kv8_alloc(pl_kv8 *c);
+void pl_kv8_release(pl_kv8 *c);
+
+/* Sequences change size: slot d_seqs[i] has d_len[i] rows from now on
+ * (d_len NULL: 0, which frees it).  Pages that a shrinking sequence leaves
+ * are released first; growing ones get the lowest free pages in the order
+ * of the list, and where one grows within a page that it shares, a copy of
+ * that page (of every layer) of its own.  All or nothing: with too few free
+ * pages nothing changes and pl_kv8_status reports PL_ENOMEM.  n <= 1024.
+ * The new rows hold nothing until they are appended. */
+int  pl_kv8_resize_dev(const pl_kv8 *c, int n, const int *d_seqs,
+                       const int *d_len, void *stream);
+
+/* Slot d_dst[i] gives up its pages and shares all of slot d_src[i]'s, the
+ * partly filled last one included (copied when one of the two grows).  A
+ * source may serve several destinations but be none.  n <= 1024. */
+int  pl_kv8_fork_dev(const pl_kv8 *c, int n, const int *d_src,
+                     const int *d_dst, void *stream);
+
+/* Move the pages in use, in order, into the free ones of lowest index, so
+ * that they occupy [0, pages in use). */
+int  pl_kv8_compact_dev(const pl_kv8 *c, void *stream);
+
+/* Copy whole pages, d_src[i] to d_dst[i], books untouched; no page may be
+ * written twice or both read and written.  n <= n_pages. */
+int  pl_kv8_copy_dev(const pl_kv8 *c, int n, const int *d_src,
+                     const int *d_dst, void *stream);
+
+/* Append: tokens d_start[i] .. d_start[i+1]-1 of k and v are the last rows
+ * of slot d_seqs[i] (which pl_kv8_resize_dev has grown; d_start NULL: one
+ * token each).  k is rotated by its row's position, then both are quantised
+ * block by block; rows that share a block with new ones are kept, rescaled
+ * if the new rows raise the block's scale.  total = d_start[n], and no entry
+ * has more than max_tok tokens.  A NaN or infinity makes its block's scale
+ * NaN, and so all of the block.  n <= 1024. */
+int  pl_kv8_append_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
+                       const int *d_start, int total, int max_tok, int dtype,
+                       const void *d_k, long long k_stride, const void *d_v,
+                       long long v_stride, void *stream);
+
+/* Causal attention: rows d_start[i] .. d_start[i+1]-1 of q are the last
+ * positions of slot d_seqs[i] (d_start NULL: one each), rotated here; token
+ * j of n_tok attends rows [0, len - n_tok + j].  A token with no row to
+ * attend gets zeros; rows of d_out past d_start[n] are left as they are. */
+int  pl_kv8_attend_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
+                       const int *d_start, int total, int max_tok, int dtype,
+                       const void *d_q, long long q_stride, void *d_out,
+                       long long out_stride, void *stream);
+
+/* A decode step: pl_kv8_append_dev and pl_kv8_attend_dev of one token for
+ * each slot. */
+int  pl_kv8_decode_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
+                       int dtype, const void *d_q, long long q_stride,
+                       const void *d_k, long long k_stride, const void *d_v,
+                       long long v_stride, void *d_out, long long out_stride,
+                       void *stream);
+
+/* Read rows back as values: rows d_row0[i] .. of slot d_seqs[i] into rows
+ * d_start[i] .. d_start[i+1]-1 of d_k and d_v (cf. pl_kv_download). */
+int  pl_kv8_read_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
+                     const int *d_row0, const int *d_start, int total,
+                     int max_rows, int dtype, void *d_k, long long k_stride,
+                     void *d_v, long long v_stride, void *stream);
+
+/* Wait for `stream`, then read and clear the cache's error word: PL_EARG,
+ * PL_ENOMEM or PL_ETIMEOUT as above, PL_OK otherwise. */
+int  pl_kv8_status(const pl_kv8 *c, void *stream);
+
 /* ---- Status and failure detection ---- */
 
 /* Wait for the work queued on `stream` (a cudaStream_t as void*; NULL = the
@@ -554,6 +740,94 @@ static inline int pl_attn_block_prefill_dev(int seq, int layer, int start_pos,
 static inline int pl_attn_proj(int layer, int which, int n, const float *x,
                                float *y) {
     (void)layer; (void)which; (void)n; (void)x; (void)y; return PL_ESTATE;
+}
+static inline int pl_rope_init(pl_rope *r, int type, int head_dim, int dim,
+                               double base, int scaling, double factor,
+                               int orig_len, double low, double high) {
+    (void)r; (void)type; (void)head_dim; (void)dim; (void)base; (void)scaling;
+    (void)factor; (void)orig_len; (void)low; (void)high; return PL_ESTATE;
+}
+static inline int pl_rope_rows_dev(const pl_rope *r, int dtype, int n,
+                                   const int *d_pos, int n_heads,
+                                   const void *d_q, long long q_stride,
+                                   void *d_q_out, long long q_out_stride,
+                                   int n_kv_heads, const void *d_k,
+                                   long long k_stride, void *d_k_out,
+                                   long long k_out_stride, int adjoint,
+                                   void *stream) {
+    (void)r; (void)dtype; (void)n; (void)d_pos; (void)n_heads; (void)d_q;
+    (void)q_stride; (void)d_q_out; (void)q_out_stride; (void)n_kv_heads;
+    (void)d_k; (void)k_stride; (void)d_k_out; (void)k_out_stride;
+    (void)adjoint; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_work_bytes(const pl_kv8 *c, size_t *bytes) {
+    (void)c; (void)bytes; return PL_ESTATE;
+}
+static inline int pl_kv8_alloc(pl_kv8 *c) {
+    (void)c; return PL_EDEVICE;
+}
+static inline void pl_kv8_release(pl_kv8 *c) {
+    (void)c;
+}
+static inline int pl_kv8_resize_dev(const pl_kv8 *c, int n, const int *d_seqs,
+                                    const int *d_len, void *stream) {
+    (void)c; (void)n; (void)d_seqs; (void)d_len; (void)stream;
+    return PL_ESTATE;
+}
+static inline int pl_kv8_fork_dev(const pl_kv8 *c, int n, const int *d_src,
+                                  const int *d_dst, void *stream) {
+    (void)c; (void)n; (void)d_src; (void)d_dst; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_compact_dev(const pl_kv8 *c, void *stream) {
+    (void)c; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_copy_dev(const pl_kv8 *c, int n, const int *d_src,
+                                  const int *d_dst, void *stream) {
+    (void)c; (void)n; (void)d_src; (void)d_dst; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_append_dev(const pl_kv8 *c, int layer, int n,
+                                    const int *d_seqs, const int *d_start,
+                                    int total, int max_tok, int dtype,
+                                    const void *d_k, long long k_stride,
+                                    const void *d_v, long long v_stride,
+                                    void *stream) {
+    (void)c; (void)layer; (void)n; (void)d_seqs; (void)d_start; (void)total;
+    (void)max_tok; (void)dtype; (void)d_k; (void)k_stride; (void)d_v;
+    (void)v_stride; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_attend_dev(const pl_kv8 *c, int layer, int n,
+                                    const int *d_seqs, const int *d_start,
+                                    int total, int max_tok, int dtype,
+                                    const void *d_q, long long q_stride,
+                                    void *d_out, long long out_stride,
+                                    void *stream) {
+    (void)c; (void)layer; (void)n; (void)d_seqs; (void)d_start; (void)total;
+    (void)max_tok; (void)dtype; (void)d_q; (void)q_stride; (void)d_out;
+    (void)out_stride; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_decode_dev(const pl_kv8 *c, int layer, int n,
+                                    const int *d_seqs, int dtype,
+                                    const void *d_q, long long q_stride,
+                                    const void *d_k, long long k_stride,
+                                    const void *d_v, long long v_stride,
+                                    void *d_out, long long out_stride,
+                                    void *stream) {
+    (void)c; (void)layer; (void)n; (void)d_seqs; (void)dtype; (void)d_q;
+    (void)q_stride; (void)d_k; (void)k_stride; (void)d_v; (void)v_stride;
+    (void)d_out; (void)out_stride; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_read_dev(const pl_kv8 *c, int layer, int n,
+                                  const int *d_seqs, const int *d_row0,
+                                  const int *d_start, int total, int max_rows,
+                                  int dtype, void *d_k, long long k_stride,
+                                  void *d_v, long long v_stride,
+                                  void *stream) {
+    (void)c; (void)layer; (void)n; (void)d_seqs; (void)d_row0; (void)d_start;
+    (void)total; (void)max_rows; (void)dtype; (void)d_k; (void)k_stride;
+    (void)d_v; (void)v_stride; (void)stream; return PL_ESTATE;
+}
+static inline int pl_kv8_status(const pl_kv8 *c, void *stream) {
+    (void)c; (void)stream; return PL_ESTATE;
 }
 static inline int pl_attn_status(void *stream) {
     (void)stream; return PL_ESTATE;

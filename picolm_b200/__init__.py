@@ -36,6 +36,12 @@ PL_ROPE_LLAMA = 0
 PL_ROPE_QWEN = 1
 PL_SPLIT_SEQS = 0
 PL_SPLIT_KV = 1
+# element types of activations, frequency scalings, formats of the 8-bit cache
+PL_F32, PL_F16, PL_BF16 = 0, 1, 2
+PL_ROPE_SCALE_NONE, PL_ROPE_SCALE_LINEAR, PL_ROPE_SCALE_YARN, PL_ROPE_SCALE_LLAMA3 = 0, 1, 2, 3
+PL_ROPE_MAX_PAIRS = 128
+PL_KV8_INT8, PL_KV8_E4M3 = 0, 1
+PL_KV8_PAGE, PL_KV8_BLOCK = 64, 16
 # GGUF tensor types the projections take (picolm/quant.h:49-63)
 PL_GGUF_F32 = 0
 PL_GGUF_F16 = 1
@@ -64,6 +70,21 @@ _vp = C.c_void_p
 _lib = None
 
 
+class _RopeStruct(C.Structure):
+    """pl_rope of include/pl_attn.h."""
+    _fields_ = [("type", C.c_int), ("head_dim", C.c_int), ("dim", C.c_int),
+                ("reserved", C.c_int), ("gain", C.c_double),
+                ("half_turns", C.c_double * PL_ROPE_MAX_PAIRS)]
+
+
+class _Kv8Struct(C.Structure):
+    """pl_kv8 of include/pl_attn.h."""
+    _fields_ = [(n, C.c_int) for n in ("device", "n_layers", "n_heads", "n_kv_heads", "head_dim",
+                                       "n_pages", "n_seqs", "max_pages", "format", "owned")] + [
+        ("rope", _RopeStruct), ("codes", _vp), ("scales", _vp), ("table", _vp), ("lens", _vp),
+        ("refs", _vp), ("work", _vp), ("work_bytes", C.c_size_t)]
+
+
 def declared_symbols() -> list[str]:
     """Names of the functions include/pl_attn.h declares (non-stub part)."""
     text = open(HEADER).read()
@@ -80,7 +101,22 @@ def load(path: str = LIB_PATH) -> C.CDLL:
         raise PlAttnError(PL_EDEVICE, f"{path} is missing; run python -m picolm_b200.build")
     lib = C.CDLL(path)
     i = C.c_int
+    ll = C.c_longlong
     sig = {
+        "pl_rope_init": (i, [_vp, i, i, i, C.c_double, i, C.c_double, i, C.c_double, C.c_double]),
+        "pl_rope_rows_dev": (i, [_vp, i, i, _vp, i, _vp, ll, _vp, ll, i, _vp, ll, _vp, ll, i, _vp]),
+        "pl_kv8_work_bytes": (i, [_vp, C.POINTER(C.c_size_t)]),
+        "pl_kv8_alloc": (i, [_vp]),
+        "pl_kv8_release": (None, [_vp]),
+        "pl_kv8_resize_dev": (i, [_vp, i, _vp, _vp, _vp]),
+        "pl_kv8_fork_dev": (i, [_vp, i, _vp, _vp, _vp]),
+        "pl_kv8_compact_dev": (i, [_vp, _vp]),
+        "pl_kv8_copy_dev": (i, [_vp, i, _vp, _vp, _vp]),
+        "pl_kv8_append_dev": (i, [_vp, i, i, _vp, _vp, i, i, i, _vp, ll, _vp, ll, _vp]),
+        "pl_kv8_attend_dev": (i, [_vp, i, i, _vp, _vp, i, i, i, _vp, ll, _vp, ll, _vp]),
+        "pl_kv8_decode_dev": (i, [_vp, i, i, _vp, i, _vp, ll, _vp, ll, _vp, ll, _vp, ll, _vp]),
+        "pl_kv8_read_dev": (i, [_vp, i, i, _vp, _vp, _vp, i, i, i, _vp, ll, _vp, ll, _vp]),
+        "pl_kv8_status": (i, [_vp, _vp]),
         "pl_attn_host_register": (i, [C.c_void_p, C.c_size_t]),
         "pl_attn_host_unregister": (i, [C.c_void_p]),
         "pl_attn_init": (i, [i, i, i, i, i, C.c_float, i, i, i]),
@@ -401,6 +437,139 @@ class Attn:
         v = _vp()
         _check(self.lib.pl_attn_kv_ptr(seq, layer, C.byref(k), C.byref(v)), "pl_attn_kv_ptr")
         return k.value, v.value
+
+
+class Rope:
+    """A rotation (pl_rope): layout, rotated elements of a head (`dim`, all
+    by default), base frequency and scaling for long contexts.  Needs no
+    device and no :class:`Attn`."""
+
+    def __init__(self, head_dim: int, rope_type: int = PL_ROPE_LLAMA, dim: int | None = None,
+                 base: float = 10000.0, scaling: int = PL_ROPE_SCALE_NONE, factor: float = 1.0,
+                 orig_len: int = 0, low: float = 1.0, high: float = 4.0):
+        self.lib = load()
+        self.struct = _RopeStruct()
+        self._p = C.addressof(self.struct)
+        _check(self.lib.pl_rope_init(self._p, rope_type, head_dim,
+                                     head_dim if dim is None else dim, base, scaling, factor,
+                                     orig_len, low, high), "pl_rope_init")
+
+    def rows_dev(self, dtype, n, d_pos, n_heads, d_q, q_stride, d_q_out, q_out_stride,
+                 n_kv_heads=0, d_k=None, k_stride=0, d_k_out=None, k_out_stride=0,
+                 adjoint=False, stream=None) -> None:
+        """Rotate n rows of q and k heads; `adjoint` for the gradient."""
+        rc = self.lib.pl_rope_rows_dev(self._p, dtype, n, d_pos, n_heads, d_q, q_stride, d_q_out,
+                                       q_out_stride, n_kv_heads, d_k, k_stride, d_k_out,
+                                       k_out_stride, 1 if adjoint else 0, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_rope_rows_dev")
+
+
+def _kv8_struct(n_layers, n_heads, n_kv_heads, head_dim, n_pages, n_seqs, max_pages, fmt, device,
+                rope):
+    c = _Kv8Struct(device=device, n_layers=n_layers, n_heads=n_heads, n_kv_heads=n_kv_heads,
+                   head_dim=head_dim, n_pages=n_pages, n_seqs=n_seqs, max_pages=max_pages,
+                   format=fmt)
+    if rope is not None:
+        c.rope = rope.struct
+    return c
+
+
+def kv8_work_bytes(n_layers: int, n_heads: int, n_kv_heads: int, head_dim: int, n_pages: int,
+                   n_seqs: int, max_pages: int, fmt: int = PL_KV8_INT8) -> int:
+    """Bytes of the workspace of a cache of this shape (pl_kv8_work_bytes)."""
+    c = _kv8_struct(n_layers, n_heads, n_kv_heads, head_dim, n_pages, n_seqs, max_pages, fmt, 0,
+                    None)
+    got = C.c_size_t()
+    _check(load().pl_kv8_work_bytes(C.addressof(c), C.byref(got)), "pl_kv8_work_bytes")
+    return got.value
+
+
+class Kv8Cache:
+    """The 8-bit paged KV cache (pl_kv8).  Without device pointers it
+    allocates its memory (and frees it on close); with them -- `codes`,
+    `scales`, `table`, `lens`, `refs`, `work`, as include/pl_attn.h lays them
+    out -- it works on an engine's own.  Needs no :class:`Attn`.  Rows are
+    device pointers with strides in elements; see the header for each call."""
+
+    def __init__(self, n_layers: int, n_heads: int, n_kv_heads: int, n_pages: int, n_seqs: int,
+                 max_pages: int, head_dim: int = HEAD_DIM, fmt: int = PL_KV8_INT8,
+                 rope: Rope | None = None, device: int = 0, codes=None, scales=None, table=None,
+                 lens=None, refs=None, work=None, work_bytes: int = 0):
+        self.lib = load()
+        self.struct = _kv8_struct(n_layers, n_heads, n_kv_heads, head_dim, n_pages, n_seqs,
+                                  max_pages, fmt, device, rope)
+        self._p = C.addressof(self.struct)
+        if codes is None:
+            _check(self.lib.pl_kv8_alloc(self._p), "pl_kv8_alloc")
+        else:
+            for name, v in (("codes", codes), ("scales", scales), ("table", table),
+                            ("lens", lens), ("refs", refs), ("work", work),
+                            ("work_bytes", work_bytes)):
+                setattr(self.struct, name, v)
+
+    def close(self) -> None:
+        self.lib.pl_kv8_release(self._p)
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        self.close()
+
+    # pages ---------------------------------------------------------------
+    def resize_dev(self, n, d_seqs, d_len=None, stream=None) -> None:
+        rc = self.lib.pl_kv8_resize_dev(self._p, n, d_seqs, d_len, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_resize_dev")
+
+    def fork_dev(self, n, d_src, d_dst, stream=None) -> None:
+        rc = self.lib.pl_kv8_fork_dev(self._p, n, d_src, d_dst, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_fork_dev")
+
+    def compact_dev(self, stream=None) -> None:
+        rc = self.lib.pl_kv8_compact_dev(self._p, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_compact_dev")
+
+    def copy_dev(self, n, d_src, d_dst, stream=None) -> None:
+        rc = self.lib.pl_kv8_copy_dev(self._p, n, d_src, d_dst, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_copy_dev")
+
+    # rows ----------------------------------------------------------------
+    def append_dev(self, layer, n, d_seqs, d_start, total, max_tok, dtype, d_k, k_stride, d_v,
+                   v_stride, stream=None) -> None:
+        rc = self.lib.pl_kv8_append_dev(self._p, layer, n, d_seqs, d_start, total, max_tok, dtype,
+                                        d_k, k_stride, d_v, v_stride, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_append_dev")
+
+    def attend_dev(self, layer, n, d_seqs, d_start, total, max_tok, dtype, d_q, q_stride, d_out,
+                   out_stride, stream=None) -> None:
+        rc = self.lib.pl_kv8_attend_dev(self._p, layer, n, d_seqs, d_start, total, max_tok, dtype,
+                                        d_q, q_stride, d_out, out_stride, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_attend_dev")
+
+    def decode_dev(self, layer, n, d_seqs, dtype, d_q, q_stride, d_k, k_stride, d_v, v_stride,
+                   d_out, out_stride, stream=None) -> None:
+        rc = self.lib.pl_kv8_decode_dev(self._p, layer, n, d_seqs, dtype, d_q, q_stride, d_k,
+                                        k_stride, d_v, v_stride, d_out, out_stride, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_decode_dev")
+
+    def read_dev(self, layer, n, d_seqs, d_row0, d_start, total, max_rows, dtype, d_k, k_stride,
+                 d_v, v_stride, stream=None) -> None:
+        rc = self.lib.pl_kv8_read_dev(self._p, layer, n, d_seqs, d_row0, d_start, total, max_rows,
+                                      dtype, d_k, k_stride, d_v, v_stride, stream)
+        if rc:
+            raise PlAttnError(rc, "pl_kv8_read_dev")
+
+    def status(self, stream=None) -> int:
+        """pl_kv8_status: wait for `stream`, read and clear the error word."""
+        return self.lib.pl_kv8_status(self._p, stream)
 
 
 def _f32(a) -> np.ndarray:

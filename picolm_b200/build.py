@@ -2,8 +2,9 @@
 
     python -m picolm_b200.build            # or: make -C picolm_b200
 
-nvcc compiles csrc/pl_attn.cu (which includes every kernel header) for
-sm_100a only and links the CUDA runtime statically.  The driver API entry
+nvcc compiles csrc/pl_attn.cu (the FP16 cache and everything around it) and
+csrc/pl_kv8.cu (rotary positions and the 8-bit paged cache), which include
+the kernel headers, for sm_100a only and links the CUDA runtime statically.  The driver API entry
 point the module needs (cuTensorMapEncodeTiled) is looked up at run time
 through cudaGetDriverEntryPoint, so the library has no link-time dependency
 on libcuda and loads on a host without a GPU (its calls then fail with
@@ -20,16 +21,17 @@ import re
 import shutil
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
-SRC = os.path.join(HERE, "csrc", "pl_attn.cu")
+SRC = [os.path.join(HERE, "csrc", f) for f in ("pl_attn.cu", "pl_kv8.cu")]
 OUT = os.path.join(HERE, "libpl_attn.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC,-O2", "-shared",
+    "-Xcompiler", "-fPIC,-O2",
     "-cudart", "static",
     "--expt-relaxed-constexpr",
 ]
@@ -103,15 +105,31 @@ def check_resources(res: dict) -> None:
 def build(force: bool = False, verbose: bool = False) -> str:
     if not force and up_to_date() and os.path.exists(RESOURCES):
         return OUT
-    cmd = [nvcc(), "-Xptxas=-v", *NVCC_FLAGS, "-I", INCLUDE, "-o", OUT, SRC]
-    if verbose:
-        print(" ".join(cmd))
-    r = subprocess.run(cmd, capture_output=True, text=True)
-    if verbose or r.returncode:
-        sys.stderr.write(r.stdout + r.stderr)
-    if r.returncode:
-        raise subprocess.CalledProcessError(r.returncode, cmd)
-    res = parse_ptxas(r.stdout + r.stderr)
+    with tempfile.TemporaryDirectory() as tmp:
+        # the translation units side by side, each with its own ptxas report
+        objs, cmds = [], []
+        for src in SRC:
+            objs.append(os.path.join(tmp, os.path.basename(src) + ".o"))
+            cmds.append([nvcc(), "-Xptxas=-v", *NVCC_FLAGS, "-I", INCLUDE, "-c", "-o", objs[-1], src])
+        runs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+                for c in cmds]
+        text = [r.communicate()[0] for r in runs]
+        cmds.append([nvcc(), *NVCC_FLAGS, "-shared", "-o", OUT, *objs])
+        codes = [r.returncode for r in runs]
+        if not any(codes):
+            r = subprocess.run(cmds[-1], capture_output=True, text=True)
+            text.append(r.stdout + r.stderr)
+            codes.append(r.returncode)
+    for cmd, out, rc in zip(cmds, text, codes):
+        if verbose:
+            print(" ".join(cmd))
+        if verbose or rc:
+            sys.stderr.write(out)
+        if rc:
+            raise subprocess.CalledProcessError(rc, cmd)
+    res = {}
+    for out in text:
+        res.update(parse_ptxas(out))
     with open(RESOURCES, "w") as f:
         json.dump(res, f, indent=1, sort_keys=True)
     check_resources(res)

@@ -1,0 +1,156 @@
+// kern_rope.cuh -- rotary positions as an operator of its own: both layouts
+// of picolm's rope() (tensor.c:537-601), part of the head, scaled
+// frequencies, FP32 / FP16 / BF16 rows, forward and adjoint.
+//
+//   y_a = x_a c - x_b s,  y_b = x_a s + x_b c,  c, s = gain * (cos, sin)(pos f_i)
+//
+// for the pairs (a, b) = (2i, 2i+1) (LLaMA) or (i, i + dim/2) (Qwen), i <
+// dim/2; elements past dim pass through.  The adjoint (the gradient with
+// respect to x) is the same with -s.  There is no table of positions: the
+// angle is taken in FP64, so a position may be any non-negative int.
+//
+// Bound by HBM: each element is read and written once (8192 rows of 32 + 8
+// heads of 128 in BF16: 168 MB).  A block rotates all heads of a few rows,
+// so that the FP64 cosines (about a hundred instructions each) are computed
+// once per (row, pair) into shared memory and not once per head.
+#pragma once
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/pl_attn.h"
+
+namespace pl {
+
+constexpr int kRopeThreads = 256;
+constexpr int kRopeRows = 8;  // rows per block, at most
+
+// cosine and sine of pair i at position pos, times the gain, rounded once
+// from FP64 to FP32
+__device__ __forceinline__ float2 rope_cs(const pl_rope& r, int i, int pos) {
+  double s, c;
+  sincospi(r.half_turns[i] * static_cast<double>(pos), &s, &c);
+  return make_float2(static_cast<float>(c * r.gain), static_cast<float>(s * r.gain));
+}
+
+// The same in FP32 after an exact reduction to [-1, 1] half turns in FP64:
+// within 2e-7 of rope_cs, at a tenth of its time.  For q, which no rounding
+// to 8 bits follows.
+__device__ __forceinline__ float2 rope_cs_fast(const pl_rope& r, int i, int pos) {
+  const double x = r.half_turns[i] * static_cast<double>(pos);
+  float s, c;
+  sincospif(static_cast<float>(x - 2.0 * rint(0.5 * x)), &s, &c);
+  const float g = static_cast<float>(r.gain);
+  return make_float2(c * g, s * g);
+}
+
+// Eight consecutive elements as FP32 (16-byte aligned FP16 / BF16, 32-byte
+// spans of FP32).
+__device__ __forceinline__ void load8(const float* p, float (&x)[8]) {
+  const float4 a = reinterpret_cast<const float4*>(p)[0], b = reinterpret_cast<const float4*>(p)[1];
+  x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+  x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+__device__ __forceinline__ void load8(const __half* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&x)[8]) {
+  const uint4 v = *reinterpret_cast<const uint4*>(p);
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    x[2 * i] = __uint_as_float(w[i] << 16);
+    x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+__device__ __forceinline__ void store8(float* p, const float (&x)[8]) {
+  reinterpret_cast<float4*>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+  reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(__half* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(x[2 * i], x[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+__device__ __forceinline__ float to_f32(float x) { return x; }
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ void from_f32(float* p, float x) { *p = x; }
+__device__ __forceinline__ void from_f32(__half* p, float x) { *p = __float2half_rn(x); }
+__device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+struct RopeRowsArgs {
+  pl_rope rope;
+  const int* pos;
+  int n, n_heads, n_kv_heads, adjoint, rows_per_block, vec;
+  const void *q, *k;
+  void *qo, *ko;
+  long long q_stride, qo_stride, k_stride, ko_stride;  // elements between rows
+};
+
+// One head row of head_dim elements by pairs: the form of any dim, stride
+// and alignment.
+template <typename T>
+__device__ __forceinline__ void rope_pair_any(const RopeRowsArgs& a, const T* x, T* y, int i,
+                                              float2 cs) {
+  const int half = a.rope.dim >> 1;
+  const int ea = a.rope.type == PL_ROPE_LLAMA ? 2 * i : i;
+  const int eb = a.rope.type == PL_ROPE_LLAMA ? 2 * i + 1 : i + half;
+  const float xa = to_f32(x[ea]), xb = to_f32(x[eb]);
+  from_f32(y + ea, __fsub_rn(__fmul_rn(xa, cs.x), __fmul_rn(xb, cs.y)));
+  from_f32(y + eb, __fadd_rn(__fmul_rn(xa, cs.y), __fmul_rn(xb, cs.x)));
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
+    const __grid_constant__ RopeRowsArgs a) {
+  __shared__ float2 s_cs[kRopeRows][PL_ROPE_MAX_PAIRS];
+  const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int rows = min(a.rows_per_block, a.n - row0);
+  for (int t = threadIdx.x; t < rows * half; t += kRopeThreads) {
+    const int r = t / half, i = t - r * half;
+    float2 cs = rope_cs(a.rope, i, a.pos[row0 + r]);
+    if (a.adjoint) cs.y = -cs.y;
+    s_cs[r][i] = cs;
+  }
+  __syncthreads();
+  const int heads = a.n_heads + a.n_kv_heads;
+  // a unit is one pair, or one element past dim, of one head
+  const int per_head = half + (hd - a.rope.dim);
+  for (int t = threadIdx.x; t < rows * heads * per_head; t += kRopeThreads) {
+    const int u = t % per_head, rh = t / per_head, h = rh % heads, r = rh / heads;
+    const bool is_q = h < a.n_heads;
+    const long long row = row0 + r;
+    const T* x = is_q ? static_cast<const T*>(a.q) + row * a.q_stride + h * hd
+                      : static_cast<const T*>(a.k) + row * a.k_stride + (h - a.n_heads) * hd;
+    T* y = is_q ? static_cast<T*>(a.qo) + row * a.qo_stride + h * hd
+                : static_cast<T*>(a.ko) + row * a.ko_stride + (h - a.n_heads) * hd;
+    if (u < half)
+      rope_pair_any<T>(a, x, y, u, s_cs[r][u]);
+    else
+      y[a.rope.dim + u - half] = x[a.rope.dim + u - half];
+  }
+}
+
+}  // namespace pl

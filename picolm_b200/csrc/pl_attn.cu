@@ -26,6 +26,7 @@
 #include "kern_prefill.cuh"
 #include "kern_proj.cuh"
 #include "kern_xfer.cuh"
+#include "pl_kv8.h"
 
 namespace {
 
@@ -205,6 +206,12 @@ cudaError_t host_alloc(T** p, size_t bytes) {
   *p = static_cast<T*>(v);
   return e;
 }
+
+}  // namespace
+
+cudaError_t pl_module::alloc(void** p, size_t bytes) { return dev_alloc(p, bytes); }
+
+namespace {
 
 int make_map(EncodeTiledFn enc, CUtensorMap* m, uint16_t* base, int head_dim, int max_seq,
              int n_kv_heads, int n_slabs, int box_rows, int box_heads) {

@@ -1,0 +1,13 @@
+// pl_kv8.h -- what pl_attn.cu and pl_kv8.cu, the two translation units of
+// libpl_attn.so, share.
+#pragma once
+#include <cstddef>
+#include <cstdint>
+#include <cuda_runtime.h>
+
+namespace pl_module {
+
+// Device allocation of the module (pl_attn.cu), with its failure injection.
+cudaError_t alloc(void** p, size_t bytes);
+
+}  // namespace pl_module

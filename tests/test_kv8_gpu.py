@@ -1,0 +1,566 @@
+"""The 8-bit paged KV cache on the GPU against plain forms in 64 bits."""
+import math
+
+import pytest
+import torch
+
+import picolm_b200 as pb
+from tests.kv8_util import (BLOCK, DTYPES, PAGE, TOP, TORCH, Cache, attention_bound, generator, i32, randn, rotate,
+                            starts, stream)
+
+pytestmark = pytest.mark.gpu
+FORMATS = (pb.PL_KV8_INT8, pb.PL_KV8_E4M3)
+
+
+# ------------------------------------------------------------------ append
+def check_rows(c, slot, first, rows, x, kv, layer=0):
+    """Rows [first, first + len(x)) of a slot hold x to half a step.
+
+    int8: |code - x / s| <= 1/2, with x / s off by the division's rounding
+    and, for k, the rotation's (8u of the block's largest value, 127 s):
+    (1/2 + 127 * 9 * 2^-24) s.  e4m3: half a step is 2^-4 of the value,
+    or 2^-10 below the smallest normal 2^-6: max(|x| 2^-4, 2^-10 s) and the same slack."""
+    got = c.values(slot, rows, layer)[kv][first:first + len(x)]
+    pages = c.table[slot, :-(-rows // PAGE)].long()
+    s = c.scales[pages, layer][:, :, kv].double()                       # [page][head][block]
+    s = s.permute(0, 2, 1).reshape(-1, c.kv_heads).repeat_interleave(BLOCK, 0)[first:first + len(x), :, None]
+    slack = TOP[c.fmt] * 9 * 2.0 ** -24 * s
+    half = 0.5 * s if c.fmt == pb.PL_KV8_INT8 else torch.maximum(x.abs() / 16, s * 2.0 ** -10)
+    assert bool(((got - x).abs() <= half + slack).all())
+    return s
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("head_dim,layout,dim", [(64, pb.PL_ROPE_LLAMA, 64), (128, pb.PL_ROPE_QWEN, 128),
+                                                 (64, pb.PL_ROPE_QWEN, 36), (128, pb.PL_ROPE_LLAMA, 10),
+                                                 (64, pb.PL_ROPE_LLAMA, 0)])
+def test_append_whole_blocks_and_tails(fmt, dtype, head_dim, layout, dim):
+    gen = generator(1)
+    counts = [1, 15, 16, 17, 64, 65, 130]
+    c = Cache(6, 3, head_dim, fmt, n_pages=16, n_seqs=8, max_pages=4, layers=2, layout=layout, rope_dim=dim)
+    seqs = [6, 0, 3, 1, 7, 2, 4]
+    c.resize(seqs, counts)
+    before = c.codes.clone()
+    rows = randn(gen, sum(counts), 2 * 3 * head_dim + 16, dtype=TORCH[dtype])
+    k, v = rows[:, :3 * head_dim], rows[:, 3 * head_dim:6 * head_dim]
+    c.append(seqs, counts, k, v, dtype, layer=1)
+    st = starts(counts)
+    for i, (slot, n) in enumerate(zip(seqs, counts)):
+        kr = rotate(k[st[i]:st[i + 1]].reshape(n, 3, head_dim), torch.arange(n, device="cuda"), c.freq, c.gain, layout)
+        vr = v[st[i]:st[i + 1]].double().reshape(n, 3, head_dim)
+        for kv, x in ((0, kr), (1, vr)):
+            s = check_rows(c, slot, 0, n, x, kv, layer=1)
+            for b in range(0, n, BLOCK):  # the scale is the block's largest value over the largest code
+                want = x[b:b + BLOCK].abs().amax((0, 2)) / TOP[fmt]
+                assert torch.allclose(s[b, :, 0], want, rtol=10 * 2.0 ** -24, atol=0)
+    # the other layer, free pages and rows past the end keep what they held
+    assert torch.equal(c.codes[:, 0], before[:, 0])
+    for slot, n in zip(seqs, counts):
+        if n % PAGE:
+            p = int(c.table[slot, n // PAGE])
+            assert torch.equal(c.codes[p, 1, :, :, n % PAGE:], before[p, 1, :, :, n % PAGE:])
+    free = c.refs == 0
+    assert torch.equal(c.codes[free], before[free])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_append_rescales_the_rows_of_its_block(fmt):
+    gen = generator(2)
+    c = Cache(4, 2, 64, fmt)
+    c.resize([0], [5])
+    k, v = randn(gen, 5, 128), randn(gen, 5, 128)
+    c.append([0], [5], k, v, pb.PL_F32)
+    old, old_s = c.values(0, 5).clone(), c.scales[int(c.table[0, 0]), 0, :, :, 0].clone()
+    codes = c.codes[int(c.table[0, 0]), 0, :, :, :5].clone()
+    c.resize([0], [6])
+    small = torch.zeros(1, 128, device="cuda")
+    c.append([0], [1], small, small, pb.PL_F32)  # a smaller row leaves the block as it is
+    assert torch.equal(c.codes[int(c.table[0, 0]), 0, :, :, :5], codes)
+    assert torch.equal(c.scales[int(c.table[0, 0]), 0, :, :, 0], old_s)
+    c.resize([0], [7])
+    big = torch.full((1, 128), 50.0, device="cuda")
+    c.append([0], [1], big, big, pb.PL_F32)
+    s = c.scales[int(c.table[0, 0]), 0, :, :, 0].double()
+    assert bool((s > old_s).all())
+    err = (c.values(0, 5) - old).abs()
+    half = (0.5 * s.t()[:, None, :, None] if fmt == pb.PL_KV8_INT8
+            else torch.maximum(old.abs() / 16, s.t()[:, None, :, None] * 2.0 ** -10))
+    assert bool((err <= half * (1 + 2.0 ** -15)).all())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_append_of_zeros_and_of_nonfinite_rows(fmt):
+    c = Cache(2, 2, 64, fmt)
+    c.resize([0, 1], [3, 20])
+    z = torch.zeros(23, 128, device="cuda")
+    z[3 + 18, 0] = math.inf   # slot 1, second block, head 0
+    z[3 + 2, 64] = math.nan   # slot 1, first block, head 1
+    c.append([0, 1], [3, 20], z, torch.zeros_like(z), pb.PL_F32)
+    assert bool((c.values(0, 3) == 0).all())
+    k, v = c.values(1, 20)
+    assert bool((v == 0).all())
+    assert bool(torch.isnan(k[16:, 0]).all()) and bool((k[:16, 0] == 0).all())
+    assert bool(torch.isnan(k[:16, 1]).all()) and bool((k[16:, 1] == 0).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_read_back(fmt, dtype):
+    gen = generator(3)
+    c = Cache(4, 4, 128, fmt, n_seqs=3)
+    c.fill([2, 0], [130, 70], gen)
+    row0, counts = [3, 69, 0], [127, 1, 0]
+    k = torch.full((130, 4 * 128 + 8), 7.0, dtype=TORCH[dtype], device="cuda")
+    v = k.clone()
+    a, b, st = i32([2, 0, 1]), i32(row0), i32(starts(counts))
+    c.c.read_dev(0, 3, a.data_ptr(), b.data_ptr(), st.data_ptr(), 128, 127, dtype, k.data_ptr(), k.stride(0),
+                 v.data_ptr(), v.stride(0), stream())
+    assert c.c.status(stream()) == pb.PL_OK
+    want = torch.cat((c.values(2, 130)[:, 3:130], c.values(0, 70)[:, 69:70]), 1).reshape(2, 128, -1)
+    # code * scale in FP32 (u = 2^-24), then one rounding to the type
+    tol = 2.0 ** -24 + (0 if dtype == pb.PL_F32 else torch.finfo(TORCH[dtype]).eps / 2 * (1 + 2.0 ** -10))
+    tiny = torch.finfo(TORCH[dtype]).tiny
+    for got, x in ((k, want[0]), (v, want[1])):
+        assert bool(((got[:128, :512].double() - x).abs() <= tol * x.abs() + tiny).all())
+        assert bool((got[128:] == 7).all()) and bool((got[:, 512:] == 7).all())
+
+
+# --------------------------------------------------------------- attention
+def attend_and_check(c, seqs, counts, dtype, gen, layer=0, q_scale=1.0):
+    total = sum(counts)
+    wide = randn(gen, total + 3, c.heads * c.head_dim + 16, dtype=TORCH[dtype])
+    q = (wide[:, :c.heads * c.head_dim] * q_scale).to(TORCH[dtype])
+    rows = torch.full((total + 3, c.heads * c.head_dim + 24), 7.0, dtype=TORCH[dtype], device="cuda")
+    out = rows[:, 8:8 + c.heads * c.head_dim]
+    c.attend(seqs, counts, q, out, dtype, layer)
+    want, most, vmax = c.reference(seqs, counts, q, layer)
+    err = (out[:total].double() - want).abs()
+    bound = attention_bound(dtype, c.head_dim, int(c.lens.max()), most, vmax, want)
+    assert bool((err <= bound).all()), float((err - bound).max())
+    assert bool((rows[total:] == 7).all()) and bool((rows[:, :8] == 7).all()) and bool((rows[:, -16:] == 7).all())
+    return out[:total], want
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("group,kv_heads", [(1, 3), (7, 2), (8, 1), (4, 4)])
+def test_one_token_at_every_kind_of_length(fmt, head_dim, group, kv_heads):
+    gen = generator(4)
+    lens = [1, 2, 15, 16, 17, 63, 64, 65, 100, 127, 128, 129, 192, 447, 511, 512]
+    c = Cache(group * kv_heads, kv_heads, head_dim, fmt, n_pages=64, n_seqs=len(lens), max_pages=8)
+    order = [int(i) for i in torch.randperm(len(lens), generator=torch.Generator().manual_seed(1))]
+    c.fill(order, lens, gen)
+    for dtype in DTYPES:
+        attend_and_check(c, order, [1] * len(lens), dtype, gen)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim,layout", [(64, pb.PL_ROPE_LLAMA), (128, pb.PL_ROPE_QWEN)])
+@pytest.mark.parametrize("counts,lens", [
+    ([2, 3, 5], [2, 70, 300]), ([17, 1, 0, 64], [17, 200, 33, 64]), ([128, 127, 129], [128, 400, 129]),
+    ([300], [512]), ([200, 256], [201, 256]), ([31, 33, 16, 47], [500, 65, 16, 512])])
+def test_several_tokens(fmt, head_dim, layout, counts, lens):
+    gen = generator(5)
+    c = Cache(8, 2, head_dim, fmt, n_pages=64, n_seqs=len(lens) + 1, max_pages=8, layout=layout)
+    seqs = list(range(len(lens), 0, -1))
+    c.fill(seqs, lens, gen)
+    for dtype in DTYPES:
+        attend_and_check(c, seqs, counts, dtype, gen)
+
+
+@pytest.mark.parametrize("group,kv_heads", [(1, 1), (3, 2), (5, 1), (6, 1), (7, 4), (8, 2), (2, 8)])
+def test_several_tokens_of_every_group(group, kv_heads):
+    gen = generator(6)
+    c = Cache(group * kv_heads, kv_heads, 64, n_pages=32, n_seqs=2, max_pages=8)
+    c.fill([0, 1], [333, 150], gen)
+    for dtype in (pb.PL_F32, pb.PL_BF16):
+        attend_and_check(c, [1, 0], [150, 77], dtype, gen)
+
+
+@pytest.mark.parametrize("counts,lens", [([1, 1], [0, 5]), ([4, 6, 3], [2, 0, 3]), ([150, 200], [20, 130])])
+def test_tokens_with_no_row_to_attend_are_zero(counts, lens):
+    """More query tokens than rows: the first ones see nothing."""
+    gen = generator(7)
+    c = Cache(8, 2, 64, n_seqs=len(lens))
+    c.fill(list(range(len(lens))), lens, gen)
+    for dtype in DTYPES:
+        out, _ = attend_and_check(c, list(range(len(lens))), counts, dtype, gen)
+        t = 0
+        for n, m in zip(counts, lens):
+            assert bool((out[t:t + max(0, n - m)] == 0).all())
+            t += n
+
+
+@pytest.mark.parametrize("count", [1, 40])
+def test_large_and_small_magnitudes(count):
+    """Scores far from 0 (one row takes all) and values far from 1: q of 1e5
+    and of 1e-6, k and v blocks from 1e-8 to 1e8."""
+    gen = generator(8)
+    c = Cache(8, 2, 64, n_seqs=1, n_pages=16)
+    c.fill([0], [300], gen)
+    pages = c.table[0, :5].long()
+    c.scales[pages, 0, :, 1] *= torch.logspace(-8, 8, 20, device="cuda").view(5, 1, 4)
+    for q_scale in (1.0, 1e-6, 1e5):
+        attend_and_check(c, [0], [count], pb.PL_F32, gen, q_scale=q_scale)
+
+
+def test_nan_stays_where_it_is():
+    """A NaN block is seen by tokens that attend it, by no others; a NaN in q
+    by its own head and token."""
+    gen = generator(9)
+    c = Cache(4, 2, 64, n_seqs=2)
+    c.fill([0, 1], [100, 100], gen)
+    c.scales[int(c.table[0, 1]), 0, 1, 0, 1] = math.nan   # rows 80..95, head 1, K
+    q = randn(gen, 200, 256)
+    q[150, 0] = math.nan
+    out = c.attend([0, 1], [100, 100], q, torch.empty_like(q), pb.PL_F32).view(200, 4, 64)
+    bad = torch.isnan(out).any(-1)
+    want = torch.zeros(200, 4, dtype=torch.bool, device="cuda")
+    want[80:100, 2:] = True
+    want[150, 0] = True
+    assert torch.equal(bad, want)
+
+
+@pytest.mark.parametrize("seqs,length", [(1, 20000), (3, 9001)])
+def test_long_contexts_are_split(seqs, length):
+    gen = generator(10)
+    c = Cache(8, 1, 64, n_pages=seqs * 320, n_seqs=seqs, max_pages=320)
+    c.fill(list(range(seqs)), [length - 777 * i for i in range(seqs)], gen)
+    for count in (1, 5, 40):
+        for dtype in (pb.PL_F32, pb.PL_BF16):
+            attend_and_check(c, list(range(seqs)), [count] * seqs, dtype, gen)
+
+
+def test_same_call_twice_gives_the_same_bits():
+    gen = generator(11)
+    c = Cache(32, 4, 64, n_pages=200, n_seqs=6, max_pages=64)
+    lens = [1, 900, 2000, 17, 333, 1500]
+    c.fill(list(range(6)), lens, gen)
+    for counts in ([1] * 6, [1, 70, 200, 9, 33, 128]):
+        q = randn(gen, sum(counts), 2048)
+        a = c.attend(list(range(6)), counts, q, torch.empty_like(q), pb.PL_F32)
+        b = c.attend(list(range(6)), counts, q, torch.empty_like(q), pb.PL_F32)
+        assert torch.equal(a, b)
+
+
+# ------------------------------------------------------------------- pages
+class Books:
+    """The page operations in plain Python."""
+
+    def __init__(self, n_pages, n_seqs):
+        self.rows, self.pages, self.refs = [0] * n_seqs, [[] for _ in range(n_seqs)], [0] * n_pages
+        self.data = list(range(n_pages))
+
+    def resize(self, seqs, lens):
+        rows, pages, refs = list(self.rows), [list(p) for p in self.pages], list(self.refs)
+        for s, m in zip(seqs, lens):
+            for p in pages[s][-(-m // PAGE):]:
+                refs[p] -= 1
+        shared = {}
+        want = []
+        for s, m in zip(seqs, lens):
+            copy = False
+            if m > rows[s] and rows[s] % PAGE:
+                p = pages[s][rows[s] // PAGE]
+                copy = refs[p] - shared.get(p, 0) > 1
+                shared[p] = shared.get(p, 0) + 1
+            want.append((copy, max(0, -(-m // PAGE) - -(-rows[s] // PAGE))))
+        free = [p for p, r in enumerate(refs) if r == 0]
+        if sum(c + n for c, n in want) > len(free):
+            return False
+        for (copy, more), s, m in zip(want, seqs, lens):
+            del pages[s][-(-m // PAGE):]
+            if copy:
+                old, pages[s][-1] = pages[s][-1], free.pop(0)
+                refs[old] -= 1
+                refs[pages[s][-1]] = 1
+                self.data[pages[s][-1]] = self.data[old]
+            for _ in range(more):
+                pages[s].append(free.pop(0))
+                refs[pages[s][-1]] = 1
+            rows[s] = m
+        self.rows, self.pages, self.refs = rows, pages, refs
+        return True
+
+    def fork(self, src, dst):
+        for a, b in zip(src, dst):
+            for p in self.pages[b]:
+                self.refs[p] -= 1
+            for p in self.pages[a]:
+                self.refs[p] += 1
+            self.pages[b], self.rows[b] = list(self.pages[a]), self.rows[a]
+
+    def compact(self):
+        used = sum(r != 0 for r in self.refs)
+        src = [p for p, r in enumerate(self.refs) if r and p >= used]
+        dst = [p for p, r in enumerate(self.refs) if not r and p < used]
+        to = dict(zip(src, dst))
+        for a, b in to.items():
+            self.refs[b], self.refs[a], self.data[b] = self.refs[a], 0, self.data[a]
+        self.pages = [[to.get(p, p) for p in s] for s in self.pages]
+
+
+def check_books(c, b):
+    assert c.lens.tolist() == b.rows
+    assert c.refs.tolist() == b.refs
+    width = c.table.shape[1]
+    assert c.table.tolist() == [p + [-1] * (width - len(p)) for p in b.pages]
+    used = [p for p, r in enumerate(b.refs) if r]
+    for p in used:  # every page in use still holds its content
+        assert bool((c.codes[p] == c.tag[b.data[p]]).all()) and bool((c.scales[p] == float(b.data[p])).all()), p
+
+
+def tagged(n_pages, n_seqs, max_pages, **kw):
+    """A cache whose page p holds the byte pattern of p."""
+    c = Cache(4, 2, 64, n_pages=n_pages, n_seqs=n_seqs, max_pages=max_pages, **kw)
+    c.tag = torch.randint(-128, 128, (n_pages,) + c.codes.shape[1:], device="cuda", generator=generator(12)).to(torch.int8)
+    c.codes.copy_(c.tag)
+    c.scales.copy_(torch.arange(n_pages, device="cuda").view(-1, 1, 1, 1, 1).expand_as(c.scales))
+    return c, Books(n_pages, n_seqs)
+
+
+@pytest.mark.parametrize("seed,layers", [(0, 1), (1, 3), (2, 2)])
+def test_pages_against_plain_books(seed, layers):
+    import random
+    r = random.Random(seed)
+    n_pages, n_seqs, max_pages = 26, 12, 9
+    c, b = tagged(n_pages, n_seqs, max_pages, layers=layers)
+    refused = 0
+    for step in range(60):
+        what = r.random()
+        k = r.randint(1, n_seqs)
+        seqs = r.sample(range(n_seqs), k)
+        if what < 0.6:
+            lens = [r.choice((0, b.rows[s], min(b.rows[s] + 1, 576), r.randint(0, 576), r.randint(0, 100))) for s in seqs]
+            ok = b.resize(seqs, lens)
+            refused += not ok
+            c.resize(seqs, lens, pb.PL_OK if ok else pb.PL_ENOMEM)
+        elif what < 0.85 and k >= 2:
+            cut = r.randint(1, k - 1)
+            src = [r.choice(seqs[:cut]) for _ in seqs[cut:]]
+            b.fork(src, seqs[cut:])
+            c.fork(src, seqs[cut:])
+        else:
+            b.compact()
+            c.compact()
+        check_books(c, b)
+    assert refused > 0
+
+
+def test_free_by_null_lengths():
+    c, b = tagged(20, 3, 8)
+    c.resize([0, 1], [200, 64])
+    b.resize([0, 1], [200, 64])
+    c.resize([1, 0])
+    b.resize([1, 0], [0, 0])
+    check_books(c, b)
+
+
+def test_one_prompt_many_continuations():
+    c, b = tagged(80, 40, 8, layers=2)
+    for cache in (c, b):
+        cache.resize([0], [130])
+        cache.fork([0] * 39, list(range(1, 40)))
+    check_books(c, b)
+    for cache in (c, b):  # slot 0 too: the last of the list keeps the shared page
+        cache.resize(list(range(39, -1, -1)), [131] * 40)
+    check_books(c, b)
+    assert sum(c.refs.tolist()) == 40 * 3 and c.refs.max() == 40
+
+
+def test_copy_pages():
+    c, _ = tagged(40, 2, 4)
+    a, b = i32([3, 9, 9, 0]), i32([39, 1, 20, 38])
+    c.c.copy_dev(4, a.data_ptr(), b.data_ptr(), stream())
+    assert c.c.status(stream()) == pb.PL_OK
+    want = list(range(40))
+    want[39], want[1], want[20], want[38] = 3, 9, 9, 0
+    for p in range(40):
+        assert bool((c.codes[p] == c.tag[want[p]]).all()) and bool((c.scales[p] == float(want[p])).all())
+    for src, dst in (([1, 2], [5, 5]), ([1, 5], [5, 6]), ([1], [40]), ([-1], [2])):
+        x, y = i32(src), i32(dst)
+        before = c.codes.clone()
+        c.c.copy_dev(len(src), x.data_ptr(), y.data_ptr(), stream())
+        assert c.c.status(stream()) == pb.PL_EARG
+        assert torch.equal(c.codes, before)
+
+
+def test_large_pools():
+    """More pages and cells than one pass of the plan's block."""
+    c = Cache(1, 1, 64, n_pages=5000, n_seqs=300, max_pages=700)
+    b = Books(5000, 300)
+    lens = [(i * 37) % 900 + (40000 if i == 7 else 0) for i in range(300)]
+    assert b.resize(list(range(300)), lens)
+    c.resize(list(range(300)), lens)
+    half = list(range(0, 300, 2))
+    b.resize(half, [0] * 150)
+    c.resize(half)
+    b.compact()
+    c.compact()
+    assert c.lens.tolist() == b.rows and c.refs.tolist() == b.refs
+    assert [[p for p in row if p >= 0] for row in c.table.tolist()] == b.pages
+
+
+# --------------------------------------------------------------- refusals
+def test_bad_entries_are_reported_and_left_undone():
+    gen = generator(13)
+    c = Cache(4, 2, 64, n_seqs=3)
+    c.fill([0, 1, 2], [40, 50, 60], gen)
+    books = [x.clone() for x in (c.table, c.lens, c.refs, c.codes)]
+
+    def same():
+        return all(torch.equal(x, y) for x, y in zip(books, (c.table, c.lens, c.refs, c.codes)))
+
+    c.resize([0, 3], [64, 64], pb.PL_EARG)
+    c.resize([0, 0], [64, 70], pb.PL_EARG)
+    c.resize([0, 1], [64, -1], pb.PL_EARG)
+    c.resize([0, 1], [64, 8 * 64 + 1], pb.PL_EARG)
+    c.resize([0], [8 * 64], pb.PL_OK)
+    c.resize([0], [40], pb.PL_OK)
+    c.fork([0, 1], [2, 2], pb.PL_EARG)
+    c.fork([0], [0], pb.PL_EARG)
+    c.fork([0, 1], [1, 2], pb.PL_EARG)
+    c.fork([0, 5], [1, 2], pb.PL_EARG)
+    assert same()
+    # attention: a slot out of range, tokens past `total`; the other entry is computed
+    q = randn(gen, 4, 256)
+    for seqs, st in (([-1, 1], [0, 1, 2]), ([7, 1], [0, 1, 2]), ([0, 1], [-1, 1, 2]), ([0, 1], [3, 2, 3])):
+        out = torch.full_like(q, 5.0)
+        a, s = i32(seqs), i32(st)
+        c.c.attend_dev(0, 2, a.data_ptr(), s.data_ptr(), 3, 2, pb.PL_F32, q.data_ptr(), 256, out.data_ptr(), 256, stream())
+        assert c.c.status(stream()) == pb.PL_EARG
+        assert c.c.status(stream()) == pb.PL_OK
+        got = out[st[1]:st[2]].double()
+        want, most, vmax = c.reference([1], [st[2] - st[1]], q[st[1]:st[2]])
+        assert bool(((got - want).abs() <= attention_bound(pb.PL_F32, 64, 64, most, vmax, want)).all())
+    # a table entry that names no page
+    c.table[1, 0] = 1000
+    out = torch.full_like(q, 5.0)
+    a = i32([1])
+    for count in (1, 2):
+        st = i32([0, count])
+        c.c.attend_dev(0, 1, a.data_ptr(), st.data_ptr(), count, count, pb.PL_F32, q.data_ptr(), 256, out.data_ptr(), 256,
+                       stream())
+        assert c.c.status(stream()) == pb.PL_EARG
+    c.c.append_dev(0, 1, a.data_ptr(), None, 1, 1, pb.PL_F32, q.data_ptr(), 256, q.data_ptr(), 256, stream())
+    assert c.c.status(stream()) == pb.PL_EARG
+    assert torch.equal(c.codes, books[3])
+
+
+def test_allocated_by_the_module(monkeypatch):
+    with pb.Kv8Cache(2, 8, 2, n_pages=10, n_seqs=2, max_pages=4) as c:
+        s, n = i32([1]), i32([70])
+        c.resize_dev(1, s.data_ptr(), n.data_ptr(), stream())
+        k = randn(generator(14), 70, 128)
+        st = i32([0, 70])
+        c.append_dev(1, 1, s.data_ptr(), st.data_ptr(), 70, 70, pb.PL_F32, k.data_ptr(), 128, k.data_ptr(), 128, stream())
+        out, zero = torch.empty(70, 128, device="cuda"), i32([0])
+        c.read_dev(1, 1, s.data_ptr(), zero.data_ptr(), st.data_ptr(), 70, 70, pb.PL_F32, out.data_ptr(), 128,
+                   out.data_ptr(), 128, stream())
+        assert c.status(stream()) == pb.PL_OK
+        # without a rotation given, rows are stored as they come: within half a step of the block's largest
+        assert float((out - k).abs().max()) <= float(k.abs().max()) / 127 * 0.51
+        with pytest.raises(pb.PlAttnError) as e:
+            c.append_dev(2, 1, s.data_ptr(), None, 1, 1, pb.PL_F32, k.data_ptr(), 128, k.data_ptr(), 128, stream())
+        assert e.value.rc == pb.PL_EARG
+    with pytest.raises(pb.PlAttnError) as e:
+        pb.Kv8Cache(1, 8, 2, n_pages=4, n_seqs=2, max_pages=4, device=63)
+    assert e.value.rc == pb.PL_EDEVICE
+
+
+# ------------------------------------------------------------ used together
+@pytest.mark.parametrize("fmt,dtype,head_dim", [(pb.PL_KV8_INT8, pb.PL_F32, 64), (pb.PL_KV8_E4M3, pb.PL_BF16, 128),
+                                                (pb.PL_KV8_INT8, pb.PL_F16, 128)])
+def test_prompt_fork_decode_and_compact_together(fmt, dtype, head_dim):
+    """A prompt in two chunks, three continuations of it, decode steps of
+    all with one ending on the way, over two layers; after each call the
+    output is that of the rows stored so far."""
+    gen = generator(15)
+    heads, kvh = 8, 2
+    c = Cache(heads, kvh, head_dim, fmt, n_pages=40, n_seqs=6, max_pages=6, layers=2, layout=pb.PL_ROPE_QWEN,
+              base=500000.0, scaling=pb.PL_ROPE_SCALE_LLAMA3, factor=8.0, orig_len=64)
+    kd = kvh * head_dim
+    plain = {}                                       # slot -> per layer [2][rows][kv heads][hd], unquantised
+
+    def step(seqs, counts, one=False):
+        lens = [int(c.lens[s]) + n for s, n in zip(seqs, counts)]
+        c.resize(seqs, lens)
+        for layer in range(2):
+            q, k, v = (randn(gen, sum(counts), w, dtype=TORCH[dtype]) for w in (heads * head_dim, kd, kd))
+            out = torch.empty_like(q)
+            if one:
+                c.decode(seqs, q, k, v, out, dtype, layer)
+            else:
+                c.append(seqs, counts, k, v, dtype, layer)
+                c.attend(seqs, counts, q, out, dtype, layer)
+            want, most, vmax = c.reference(seqs, counts, q, layer)
+            assert bool(((out.double() - want).abs() <= attention_bound(dtype, head_dim, max(lens), most, vmax, want)).all())
+            t = 0
+            for s, n, m in zip(seqs, counts, lens):
+                kr = rotate(k[t:t + n].view(n, kvh, head_dim), torch.arange(m - n, m, device="cuda"), c.freq, c.gain,
+                            c.layout)
+                new = torch.stack((kr, v[t:t + n].double().view(n, kvh, head_dim)))
+                had = plain.get((s, layer), new[:, :0])
+                plain[s, layer] = torch.cat((had, new), 1)
+                t += n
+
+    step([0], [70])
+    step([0], [58])
+    step([3], [9])
+    c.fork([0, 0, 0], [1, 2, 4])
+    for s in (1, 2, 4):
+        for layer in range(2):
+            plain[s, layer] = plain[0, layer]
+    for i in range(20):
+        step([4, 0, 3, 1, 2] if i < 9 else [4, 0, 2], [1] * (5 if i < 9 else 3), one=True)
+        if i == 8:
+            c.resize([3, 1])
+            c.compact()
+            used = int((c.refs > 0).sum())
+            assert bool((c.refs[:used] > 0).all())
+    # what is stored is within the steps of its format of what was appended:
+    # half a step for the rounding, and half a step more for each of up to
+    # 15 later rows that raised the scale of its block
+    for s in (0, 2, 4):
+        for layer in range(2):
+            got, x = c.values(s, plain[s, layer].shape[1], layer), plain[s, layer]
+            top = float(x.abs().max())
+            limit = 8 * top / 127 if fmt == pb.PL_KV8_INT8 else 8 * torch.maximum(x.abs() / 16, torch.full_like(x, top / 448 / 1024)) * 1.5
+            assert bool(((got - x).abs() <= limit).all())
+
+
+def test_captured_step_replayed():
+    """A step (grow, append, attend) captured in a graph on another stream
+    and replayed: every replay appends the next token."""
+    gen = generator(16)
+    c = Cache(8, 2, 64, n_pages=32, n_seqs=3, max_pages=8)
+    c.fill([0, 1, 2], [60, 1, 127], gen)
+    lens, seqs = i32([60, 1, 127]), i32([0, 1, 2])
+    q, k, v = randn(gen, 3, 512), randn(gen, 3, 128), randn(gen, 3, 128)
+    out = torch.zeros_like(q)
+
+    def one():
+        lens.add_(1)
+        c.c.resize_dev(3, seqs.data_ptr(), lens.data_ptr(), stream())
+        c.c.decode_dev(0, 3, seqs.data_ptr(), pb.PL_F32, q.data_ptr(), 512, k.data_ptr(), 128, v.data_ptr(), 128,
+                       out.data_ptr(), 512, stream())
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        one()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        one()
+    for i in range(6):
+        q.copy_(randn(gen, 3, 512))
+        k.copy_(randn(gen, 3, 128))
+        v.copy_(randn(gen, 3, 128))
+        graph.replay()
+        assert c.c.status(stream()) == pb.PL_OK
+        assert c.lens.tolist() == [60 + i + 2, 1 + i + 2, 127 + i + 2]
+        want, most, vmax = c.reference([0, 1, 2], [1, 1, 1], q)
+        assert bool(((out.double() - want).abs() <= attention_bound(pb.PL_F32, 64, 140, most, vmax, want)).all())
+    del graph
