@@ -152,13 +152,6 @@ __device__ __forceinline__ float2 rope_two(const float* x, int d, const float* c
   return y;
 }
 
-// Split an FP32 pair into FP16 high parts and FP16 residuals.
-__device__ __forceinline__ void split_hi_lo(float a, float b, uint32_t& hi, uint32_t& lo) {
-  hi = pack_half2(a, b);
-  const float2 h = unpack_half2(hi);
-  lo = pack_half2(a - h.x, b - h.y);
-}
-
 // Byte offset of 16-byte chunk `chunk` of row `r` in a 128-byte-swizzled
 // tile (rows of 128 bytes, 1024-byte aligned base): TMA's SWIZZLE_128B.
 __device__ __forceinline__ uint32_t sw128(int r, int chunk) {

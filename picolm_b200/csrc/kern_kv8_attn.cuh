@@ -119,4 +119,602 @@ __global__ void __launch_bounds__(kPlainThreads) kv8_attend_plain_kernel(
     for (int gq = 0; gq < G; ++gq) from_f32(out + gq * HD + tid, o[gq] / s_l[gq]);
 }
 
+// ------------------------------------------------------- one token a slot
+// Bound by HBM: 2 * head_dim + 0.5 bytes a row and KV head.
+//
+// Work partition.  A tile is kTileRows rows of one page and KV head, 4 KB of
+// K and 4 KB of V.  The tiles of all entries, (entry, head, tile) in order,
+// form one list; every block takes an equal contiguous slice of it and every
+// warp of the block one of that, whatever the lengths are.  The part of one
+// (entry, head) -- a run -- inside a warp's slice is a segment.
+//
+// Each warp is on its own: its first lane streams the warp's tiles through a
+// ring of kStages 8 KB stages (tiled TMA loads, swizzled by the width of a
+// row so that ldmatrix is free of bank conflicts), and the whole warp
+// consumes them, so no warp waits for another until its slice is done.
+//
+// Scores and P.V run on mma.sync (m16n8k16, FP16 in, FP32 out): on CUDA
+// cores the dot products alone would need more issue slots than HBM leaves.
+// Every code is exact in FP16.  ldmatrix moves the bytes as 16-bit pairs:
+// without .trans a thread gets bytes 4c .. 4c+3 of a row's 16-byte chunk, so
+// K step j of Q K^T holds the dims 16j + 4c + {0, 1, 2, 3} in its slots 2c,
+// 2c+1, 2c+8, 2c+9 (q is laid out the same way); with .trans it gets bytes 2g, 2g+1
+// of rows 2c, 2c+1, so two n-tiles of P V hold the even and the odd dims of
+// a chunk.  Rows 0..7 of the A operand hold the FP16 high part of q (of the
+// weights), rows 8..15 the residual, which costs nothing in an m16 tile of
+// at most 8 heads and carries FP32 inputs to 2^-22.
+//
+// Ranges.  q is scaled by the power of two that puts its row's largest
+// element into [1, 2); weights are 2^(s - m) * sv * 2^14 / ref with ref the
+// largest V scale so far, so that residuals stay above FP16's smallest
+// subnormals (a weight of 2^-20 still has 18 bits) and nothing overflows.
+// Each tile's P V starts from zero and is added to the running output with
+// one rounded FP32 FMA: the tensor core truncates as it accumulates, and
+// over a long segment that would add up in one direction.
+//
+// Segments of a run in several warps of a block are merged in shared
+// memory by the warp where the run starts; runs over several blocks leave
+// one partial a block in the workspace, and the block that finishes a run's
+// last partial merges them, in the order of the blocks.
+constexpr int kDecWarps = 8;
+constexpr int kDecThreads = kDecWarps * 32;
+constexpr int kDecTileBytes = 4096;  // of K, and of V
+constexpr float kWeightScale = 16384.f;
+constexpr float kMinRef = 1e-30f;
+
+template <int HD>
+struct DecShape {
+  static constexpr int kTileRows = kDecTileBytes / HD;    // 64 or 32
+  static constexpr int kTilesPerPage = kPage / kTileRows;
+  static constexpr int kBlocks = kTileRows / kBlock;      // scales in a tile
+  static constexpr int kStages = HD == 64 ? 3 : 2;
+  static constexpr int kPartFloats = 32 * (HD / 4 + 2);   // a partial: lane-wise m, l, o
+};
+
+template <int HD>
+struct DecSmem {
+  using Sh = DecShape<HD>;
+  uint8_t ring[kDecWarps][Sh::kStages][2][kDecTileBytes];  // 1024-byte aligned
+  float scales[kDecWarps][Sh::kStages][2][kBlocksPerPage];
+  float part[kDecWarps][Sh::kPartFloats];
+  float2 cs[kDecWarps][HD / 2];
+  uint64_t full[kDecWarps][Sh::kStages];
+  int prefix[kPlanSeqs + 1];
+  int warp_sum[kDecWarps];
+  int finish[2];
+};
+
+struct Kv8DecodeArgs {
+  Kv8AttnArgs a;
+  float* part;    // [2 * blocks][kPartFloats]
+  int* arrived;   // [entries * kv heads], zero at rest
+};
+
+// Four consecutive elements (16-byte aligned FP32, 8-byte aligned 16-bit).
+__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+  const float4 v = *reinterpret_cast<const float4*>(p);
+  x[0] = v.x, x[1] = v.y, x[2] = v.z, x[3] = v.w;
+}
+__device__ __forceinline__ void load4(const __half* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  const float2 a = unpack_half2(v.x), b = unpack_half2(v.y);
+  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
+}
+__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
+  const uint2 v = *reinterpret_cast<const uint2*>(p);
+  x[0] = __uint_as_float(v.x << 16), x[1] = __uint_as_float(v.x & 0xffff0000u);
+  x[2] = __uint_as_float(v.y << 16), x[3] = __uint_as_float(v.y & 0xffff0000u);
+}
+__device__ __forceinline__ void store4(float* p, const float (&x)[4]) {
+  *reinterpret_cast<float4*>(p) = make_float4(x[0], x[1], x[2], x[3]);
+}
+__device__ __forceinline__ void store4(__half* p, const float (&x)[4]) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]));
+}
+__device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
+  const __nv_bfloat162 a = __floats2bfloat162_rn(x[0], x[1]), b = __floats2bfloat162_rn(x[2], x[3]);
+  *reinterpret_cast<uint2*>(p) = make_uint2(*reinterpret_cast<const uint32_t*>(&a),
+                                            *reinterpret_cast<const uint32_t*>(&b));
+}
+
+// Elements [e, e + 4) of a head row, rotated (e a multiple of 4).
+template <typename T>
+__device__ __forceinline__ void load_rotated4(const T* x, int e, const pl_rope& r, const float2* cs,
+                                              float (&y)[4]) {
+  load4(x + e, y);
+  if (e >= r.dim) return;
+  const int half = r.dim >> 1;
+  if (r.type == PL_ROPE_LLAMA) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (e + 2 * j >= r.dim) break;
+      const float2 c = cs[(e >> 1) + j];
+      const float a = y[2 * j], b = y[2 * j + 1];
+      y[2 * j] = a * c.x - b * c.y;
+      y[2 * j + 1] = a * c.y + b * c.x;
+    }
+  } else if (half % 4 == 0) {
+    const bool first = e < half;
+    float z[4];
+    load4(x + (first ? e + half : e - half), z);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float2 c = cs[(first ? e : e - half) + j];
+      y[j] = first ? y[j] * c.x - z[j] * c.y : z[j] * c.y + y[j] * c.x;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int d = e + j;
+      if (d >= r.dim) break;
+      if (d < half) {
+        y[j] = y[j] * cs[d].x - to_f32(x[d + half]) * cs[d].y;
+      } else {
+        y[j] = to_f32(x[d - half]) * cs[d - half].y + y[j] * cs[d - half].x;
+      }
+    }
+  }
+}
+
+// Codes as FP16 pairs.  int8: the byte with its sign bit flipped below a
+// 0x64 is 1024 + 128 + code in FP16; e4m3 converts in hardware.
+template <int FMT, int SEL>
+__device__ __forceinline__ uint32_t codes_half2(uint32_t w) {
+  // bytes a, b of w with SEL = a | b << 4
+  if constexpr (FMT == PL_KV8_INT8) {
+    constexpr uint32_t sel = (SEL & 0xf) | 0x40 | ((SEL >> 4) << 8) | 0x4000;
+    const uint32_t h = __byte_perm(w ^ 0x80808080u, 0x64646464u, sel);
+    uint32_t d;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(h), "r"(0x64806480u));
+    return d;
+  } else {
+    constexpr uint32_t sel = (SEL & 0xf) | (SEL & 0xf0);
+    uint32_t d;
+    const uint16_t two = static_cast<uint16_t>(sel == 0x10 ? w : __byte_perm(w, 0u, sel | 0x4400u));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(d) : "h"(two));
+    return d;
+  }
+}
+
+// Byte offset of 16-byte chunk `ch` of row r in a tile of HD-byte rows, as
+// the TMA swizzle of that width places it.
+template <int HD>
+__device__ __forceinline__ uint32_t tile_off(int r, int ch) {
+  if constexpr (HD == 64) return r * 64 + ((ch ^ ((r >> 1) & 3)) << 4);
+  return r * 128 + ((ch ^ (r & 7)) << 4);
+}
+
+// The list of tiles: prefix sums over entries, in tiles of all heads.
+template <int HD>
+struct DecWork {
+  const int* prefix;
+  int n, heads;
+  int total, blocks;  // tiles; blocks that hold work
+  __device__ __forceinline__ int begin(int b) const {
+    return static_cast<int>(static_cast<long long>(b) * total / blocks);
+  }
+  // the block that owns tile x: the largest b with begin(b) <= x
+  __device__ __forceinline__ int block_of(int x) const {
+    return static_cast<int>(((static_cast<long long>(x) + 1) * blocks - 1) / total);
+  }
+  __device__ __forceinline__ int entry_of(int x) const {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid + 1] > x) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  }
+};
+
+// Running state of a segment: row g = lane / 4 of the A operand is query
+// head g of the KV head, this thread holds its dims 16ch + 4(lane % 4) ..
+template <int HD>
+struct DecState {
+  float m, l, o[HD / 4];
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) o[i] = 0.f;
+  }
+  __device__ __forceinline__ void fold(float m2, float l2, const float (&o2)[HD / 4]) {
+    const float mx = fmaxf(m, m2);
+    if (mx == -INFINITY) {  // neither has a row (or one holds NaN)
+      l += l2;
+      return;
+    }
+    const float a = ex2(m - mx), b = ex2(m2 - mx);
+    l = l * a + l2 * b;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) o[i] = o[i] * a + o2[i] * b;
+    m = mx;
+  }
+  __device__ __forceinline__ void save(float* p, int lane) const {
+    p[lane] = m;
+    p[32 + lane] = l;
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) p[(2 + i) * 32 + lane] = o[i];
+  }
+  __device__ __forceinline__ void fold_from(const float* p, int lane) {
+    float o2[HD / 4];
+    const float m2 = p[lane], l2 = p[32 + lane];
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) o2[i] = p[(2 + i) * 32 + lane];
+    fold(m2, l2, o2);
+  }
+  template <typename T>
+  __device__ __forceinline__ void write(T* out, int lane, int group) const {
+    const int g = lane >> 2, c = lane & 3;
+    if (g >= group) return;
+    const float inv = 1.0f / l;
+#pragma unroll
+    for (int ch = 0; ch < HD / 16; ++ch) {
+      const float x[4] = {o[4 * ch] * inv, o[4 * ch + 1] * inv, o[4 * ch + 2] * inv,
+                          o[4 * ch + 3] * inv};
+      store4(out + g * HD + 16 * ch + 4 * c, x);
+    }
+  }
+};
+
+template <typename T, int HD, int FMT>
+__global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
+    const __grid_constant__ Kv8DecodeArgs da, const __grid_constant__ CUtensorMap tm) {
+  using Sh = DecShape<HD>;
+  constexpr int NS = Sh::kStages, TR = Sh::kTileRows;
+  extern __shared__ uint8_t smem_raw[];
+  DecSmem<HD>& sm = *reinterpret_cast<DecSmem<HD>*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  const Kv8AttnArgs& a = da.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int g = lane >> 2, c = lane & 3;
+  const int heads = a.g.n_kv_heads, G = a.group;
+  if (lane == 0) {
+    for (int s = 0; s < NS; ++s) mbar_init(&sm.full[warp][s], 1);
+    fence_mbar_init();
+    if (warp == 0) tma_prefetch_desc(&tm);
+  }
+  __syncwarp();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- tiles of every entry, scanned
+  {
+    const int per = (a.n + kDecThreads - 1) / kDecThreads, i0 = tid * per;
+    int mine = 0;
+    bool bad = false;
+    for (int i = i0; i < min(a.n, i0 + per); ++i) {
+      Kv8Entry e;
+      const bool ok = kv8_entry(a.g, i, a.total, 1, a.seqs, a.start, e);
+      bad |= !ok;
+      const int rows = ok && e.n_tok ? e.len : 0;
+      const int tiles = (rows + TR - 1) / TR * heads;
+      sm.prefix[i] = tiles;
+      mine += tiles;
+      // nothing to attend: zeros
+      if (ok && e.n_tok && e.len == 0 && blockIdx.x == 0)
+        for (int d = 0; d < a.n_heads * HD; ++d)
+          from_f32(static_cast<T*>(a.out) + e.tok0 * a.out_stride + d, 0.f);
+    }
+    if (bad && blockIdx.x == 0) atomicOr(&a.g.head->err, ERR_BAD_ARG);
+    int x = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, d);
+      if (lane >= d) x += y;
+    }
+    if (lane == 31) sm.warp_sum[warp] = x;
+    __syncthreads();
+    int base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+      base += w < warp ? sm.warp_sum[w] : 0;
+      total += sm.warp_sum[w];
+    }
+    int run = base + x - mine;
+    for (int i = i0; i < min(a.n, i0 + per); ++i) {
+      const int t = sm.prefix[i];
+      sm.prefix[i] = run;
+      run += t;
+    }
+    if (tid == 0) {
+      sm.prefix[a.n] = total;
+      sm.finish[0] = sm.finish[1] = -1;
+    }
+    __syncthreads();
+  }
+  const int total = sm.prefix[a.n];
+  const DecWork<HD> work{sm.prefix, a.n, heads, total, min(static_cast<int>(gridDim.x), total)};
+  const int blk = blockIdx.x;
+  if (blk >= work.blocks) return;
+  const int b0 = work.begin(blk), b1 = work.begin(blk + 1), span = b1 - b0;
+  const int x0 = b0 + static_cast<int>(static_cast<long long>(warp) * span / kDecWarps);
+  const int x1 = b0 + static_cast<int>(static_cast<long long>(warp + 1) * span / kDecWarps);
+
+  // ---- this warp's tiles: 32 at a time, tile x0 + 32k + lane in this lane
+  int t_run = 0, t_row = 0, t_slab = 0, t_len = 0, t_base = x0 - 32;
+  auto fetch_tiles = [&](int base) {
+    t_base = base;
+    const int x = base + lane;
+    if (x < x1) {
+      const int i = work.entry_of(x);
+      const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
+      const int rem = x - sm.prefix[i], h = rem / tiles, t = rem - h * tiles;
+      const int slot = a.seqs[i];
+      int page = a.g.table[static_cast<long long>(slot) * a.g.max_pages + t / Sh::kTilesPerPage];
+      t_len = a.g.lens[slot];
+      if (page < 0 || page >= a.g.n_pages) {
+        atomicOr(&a.g.head->err, ERR_BAD_ARG);
+        page = 0;
+      }
+      t_run = i * heads + h;
+      t_row = t * TR;
+      t_slab = static_cast<int>(a.g.slab(page, h, 0));
+    }
+  };
+  auto issue = [&](int x, int slab, int row) {  // lane 0
+    const int s = (x - x0) % NS;
+    uint64_t* bar = &sm.full[warp][s];
+    mbar_arrive_expect_tx(bar, 2 * kDecTileBytes + 2 * kBlocksPerPage * 4);
+    tma_load_3d(sm.ring[warp][s][0], &tm, bar, 0, row % kPage, slab);
+    tma_load_3d(sm.ring[warp][s][1], &tm, bar, 0, row % kPage, slab + 1);
+    bulk_load(sm.scales[warp][s], a.g.scales + static_cast<long long>(slab) * kBlocksPerPage,
+              2 * kBlocksPerPage * 4, bar);
+  };
+  bool ok = true;
+  int issued = x0;
+  if (x0 < x1) fetch_tiles(x0);
+  for (; issued < x1 && issued < x0 + NS; ++issued) {
+    const int slab = __shfl_sync(0xffffffffu, t_slab, issued - t_base);
+    const int row = __shfl_sync(0xffffffffu, t_row, issued - t_base);
+    if (lane == 0) issue(issued, slab, row);
+  }
+
+  uint32_t qa[HD / 16][4];
+  DecState<HD> st;
+  st.clear();
+  // This block's partial of a run over several blocks (kind 0: the run
+  // started before the block, 1: in it); the last block to leave one is to
+  // merge them.
+  auto publish = [&](int r, int first, int last, int kind) {
+    st.save(da.part + static_cast<long long>(2 * blk + kind) * Sh::kPartFloats, lane);
+    __threadfence();
+    __syncwarp();
+    if (lane == 0) {
+      const int parts = work.block_of(last) - work.block_of(first) + 1;
+      if (atomicAdd(&da.arrived[r], 1) == parts - 1) {
+        da.arrived[r] = 0;
+        __threadfence();
+        sm.finish[kind] = r;
+      }
+    }
+    __syncwarp();
+  };
+  float ref = kMinRef, q_scale = 0.f;
+  int run = -1, run_first = 0, run_last = 0;  // the current run and its tiles
+  const uint32_t ring = smem_u32(sm.ring[warp]);
+  // tile fields of the consumed tile live one batch behind the issued ones
+  int c_run = t_run, c_row = t_row, c_len = t_len, c_base = t_base;
+  for (int x = x0; x < x1 && ok; ++x) {
+    if (x - c_base >= 32) {
+      c_run = t_run, c_row = t_row, c_len = t_len, c_base = t_base;
+    }
+    const int x_run = __shfl_sync(0xffffffffu, c_run, x - c_base);
+    const int row0 = __shfl_sync(0xffffffffu, c_row, x - c_base);
+    const int len = __shfl_sync(0xffffffffu, c_len, x - c_base);
+    const int i = x_run / heads, h = x_run - i * heads;
+    if (x_run != run) {
+      // ---- a new run: its query rows
+      run = x_run;
+      const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
+      run_first = sm.prefix[i] + h * tiles;
+      run_last = run_first + tiles - 1;
+      const int tok = a.start ? a.start[i] : i;
+      for (int p = lane; p < a.rope.dim >> 1; p += 32)
+        sm.cs[warp][p] = rope_cs_fast(a.rope, p, len - 1);
+      __syncwarp();
+      const T* q = static_cast<const T*>(a.q) + tok * a.q_stride + (h * G + min(g, G - 1)) * HD;
+      float y[HD / 16][4], top = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j) {
+        load_rotated4(q, 16 * j + 4 * c, a.rope, sm.cs[warp], y[j]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(y[j][e]));
+      }
+      __syncwarp();
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^-e with 2^e <= top < 2^(e+1), for normal finite tops
+      const uint32_t ex = __float_as_uint(top) >> 23;
+      const bool norm = ex > 1 && ex < 253;
+      const float down = norm ? __uint_as_float((254u - ex) << 23) : 1.f;
+      q_scale = (norm ? __uint_as_float(ex << 23) : 1.f) * a.score_scale;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const float u = g < G ? y[j][2 * hf] * down : 0.f;
+          const float v = g < G ? y[j][2 * hf + 1] * down : 0.f;
+          split_hi_lo(u, v, qa[j][2 * hf], qa[j][2 * hf + 1]);
+        }
+      st.clear();
+      ref = kMinRef;
+    }
+    const int s = (x - x0) % NS;
+    if (!mbar_wait_bounded(&sm.full[warp][s], ((x - x0) / NS) & 1)) {
+      if (lane == 0) atomicOr(&a.g.head->err, ERR_TIMEOUT_FULL);
+      ok = false;
+      break;
+    }
+    const uint32_t kt = ring + s * 2 * kDecTileBytes, vt = kt + kDecTileBytes;
+    const float* sk = sm.scales[warp][s][0] + row0 % kPage / kBlock;
+    const float* sv = sm.scales[warp][s][1] + row0 % kPage / kBlock;
+    // ---- S = Q K^T
+    float sc[TR / 8][4];
+#pragma unroll
+    for (int nt = 0; nt < TR / 8; ++nt) {
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+#pragma unroll
+      for (int q4 = 0; q4 < HD / 64; ++q4) {
+        uint32_t w[4];
+        ldmatrix_x4(kt + tile_off<HD>(nt * 8 + (lane & 7), 4 * q4 + (lane >> 3)), w[0], w[1], w[2],
+                    w[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          mma_16816(sc[nt], qa[4 * q4 + j], codes_half2<FMT, 0x10>(w[j]),
+                    codes_half2<FMT, 0x32>(w[j]));
+      }
+    }
+    const bool tail = row0 + TR > len;
+    float mt = -INFINITY;
+#pragma unroll
+    for (int nt = 0; nt < TR / 8; ++nt) {
+      const float by = q_scale * sk[nt / 2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float v = (sc[nt][e] + sc[nt][2 + e]) * by;
+        if (tail && row0 + nt * 8 + 2 * c + e >= len) v = -INFINITY;
+        sc[nt][e] = v;
+        mt = fmaxf(mt, v);
+      }
+    }
+    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+    mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+    const float m_new = fmaxf(st.m, mt);
+    const float alpha = ex2(st.m - m_new);
+    float top = sv[0];
+#pragma unroll
+    for (int b = 1; b < Sh::kBlocks; ++b)
+      if (row0 + b * kBlock < len) top = fmaxf(top, sv[b]);
+    const float ref_new = fmaxf(ref, top);
+    const float keep = alpha * (ref / ref_new), lift = kWeightScale / ref_new;
+    ref = ref_new;
+    st.m = m_new;
+    st.l *= alpha;
+    // ---- O = O * keep + P V
+    float ot[HD / 8][4];
+#pragma unroll
+    for (int j = 0; j < HD / 8; ++j) ot[j][0] = ot[j][1] = ot[j][2] = ot[j][3] = 0.f;
+#pragma unroll
+    for (int b = 0; b < Sh::kBlocks; ++b) {
+      if (row0 + b * kBlock >= len) break;
+      const float by = sv[b] * lift;
+      uint32_t pa[4];
+#pragma unroll
+      for (int hf = 0; hf < 2; ++hf) {
+        const float p0 = ex2(sc[2 * b + hf][0] - m_new), p1 = ex2(sc[2 * b + hf][1] - m_new);
+        st.l += p0 + p1;
+        split_hi_lo(p0 * by, p1 * by, pa[2 * hf], pa[2 * hf + 1]);
+      }
+      // rows past the end weigh 0, but their bytes may be NaN codes
+      uint32_t seen0 = 0xffffffffu, seen1 = 0xffffffffu;
+      if (tail) {
+        const int r = row0 + b * kBlock + 2 * c;
+        seen0 = (r < len ? 0xffffu : 0u) | (r + 1 < len ? 0xffff0000u : 0u);
+        seen1 = (r + 8 < len ? 0xffffu : 0u) | (r + 9 < len ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int ch = 0; ch < HD / 16; ch += 2) {
+        uint32_t w[4];  // (rows 0-7, 8-15) of chunk ch, then of ch + 1
+        ldmatrix_x4_trans(vt + tile_off<HD>(b * kBlock + ((lane >> 3) & 1) * 8 + (lane & 7),
+                                            ch + (lane >> 4)),
+                          w[0], w[1], w[2], w[3]);
+        w[0] &= seen0, w[1] &= seen1, w[2] &= seen0, w[3] &= seen1;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          mma_16816(ot[2 * (ch + k)], pa, codes_half2<FMT, 0x20>(w[2 * k]),
+                    codes_half2<FMT, 0x20>(w[2 * k + 1]));
+          mma_16816(ot[2 * (ch + k) + 1], pa, codes_half2<FMT, 0x31>(w[2 * k]),
+                    codes_half2<FMT, 0x31>(w[2 * k + 1]));
+        }
+      }
+    }
+    // n-tiles 2ch, 2ch+1 hold the dims 16ch + 4c + {0, 2} and {1, 3}
+#pragma unroll
+    for (int ch = 0; ch < HD / 16; ++ch)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float* t = ot[2 * ch + (e & 1)];
+        st.o[4 * ch + e] = fmaf(st.o[4 * ch + e], keep, t[e >> 1] + t[2 + (e >> 1)]);
+      }
+    // ---- the stage is free: the next tile
+    __syncwarp();
+    if (issued < x1) {
+      if (issued - t_base >= 32) fetch_tiles(issued);
+      const int slab = __shfl_sync(0xffffffffu, t_slab, issued - t_base);
+      const int row = __shfl_sync(0xffffffffu, t_row, issued - t_base);
+      if (lane == 0) issue(issued, slab, row);
+      ++issued;
+    }
+    // ---- the segment's end
+    if (x == run_last || x == x1 - 1) {
+      st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+      st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+      const float back = ref * (1.f / kWeightScale);
+#pragma unroll
+      for (int d = 0; d < HD / 4; ++d) st.o[d] *= back;
+      if (max(run_first, b0) < x0) {
+        st.save(sm.part[warp], lane);  // the warp where the run starts takes it
+      } else if (x == run_last && run_first >= b0) {
+        const int tok = a.start ? a.start[i] : i;
+        st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
+      } else if (x != x1 - 1) {
+        publish(run, run_first, run_last, 0);  // the end of an earlier block's run
+      }
+    }
+  }
+  // never leave with copies in flight
+  for (int x = max(issued - NS, x0); x < issued; ++x)
+    mbar_wait_bounded(&sm.full[warp][(x - x0) % NS], ((x - x0) / NS) & 1);
+  __syncthreads();
+
+  // ---- runs that go on past this warp's slice (or came from another block):
+  // the warp where the block's part of the run starts folds in the others'
+  const bool mine = ok && x0 < x1 && max(run_first, b0) >= x0 &&
+                    (run_last >= x1 || run_first < b0);
+  if (mine) {
+    const int end = min(run_last + 1, b1);
+    for (int w = warp + 1; w < kDecWarps; ++w) {
+      const int w0 = b0 + static_cast<int>(static_cast<long long>(w) * span / kDecWarps);
+      const int w1 = b0 + static_cast<int>(static_cast<long long>(w + 1) * span / kDecWarps);
+      if (w0 < w1 && w0 < end) st.fold_from(sm.part[w], lane);
+    }
+    const int i = run / heads, h = run - i * heads;
+    if (run_first >= b0 && run_last < b1) {
+      const int tok = a.start ? a.start[i] : i;
+      st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
+    } else {
+      publish(run, run_first, run_last, run_first >= b0 ? 1 : 0);
+    }
+  }
+  __syncthreads();
+  // ---- the last of a run's blocks merges its partials, all warps together
+#pragma unroll 1
+  for (int f = 0; f < 2; ++f) {
+    const int r = sm.finish[f];
+    if (r < 0) continue;
+    const int i = r / heads, h = r - i * heads;
+    const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
+    const int first = sm.prefix[i] + h * tiles, f0 = work.block_of(first);
+    const int parts = work.block_of(first + tiles - 1) - f0 + 1;
+    st.clear();
+    for (int p = warp; p < parts; p += kDecWarps) {
+      const int slot = 2 * (f0 + p) + (first >= work.begin(f0 + p) ? 1 : 0);
+      const float* src = da.part + static_cast<long long>(slot) * Sh::kPartFloats;
+      float o2[HD / 4];
+      const float m2 = __ldcg(src + lane), l2 = __ldcg(src + 32 + lane);
+#pragma unroll
+      for (int d = 0; d < HD / 4; ++d) o2[d] = __ldcg(src + (2 + d) * 32 + lane);
+      st.fold(m2, l2, o2);
+    }
+    st.save(sm.part[warp], lane);
+    __syncthreads();
+    if (warp == 0) {
+      for (int w = 1; w < kDecWarps; ++w) st.fold_from(sm.part[w], lane);
+      const int tok = a.start ? a.start[i] : i;
+      st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
+    }
+    __syncthreads();
+  }
+}
+
 }  // namespace pl

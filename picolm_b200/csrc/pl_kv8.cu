@@ -4,6 +4,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cmath>
 #include <cstdio>
 #include <cstring>
@@ -66,6 +67,61 @@ int sm_count() {
   return n;
 }
 
+// Blocks of a one-token attention grid, at most (the workspace holds two
+// partials for each).
+constexpr int kMaxBlocks = 160;
+
+// Shared memory above 48 KB is an attribute of a kernel on each device: set
+// the first time this kernel launches there.
+template <typename K>
+int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
+  int dev = 0;
+  PL_CUDA(cudaGetDevice(&dev));
+  const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
+  if (bit && (done.load(std::memory_order_acquire) & bit)) return PL_OK;
+  PL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  done.fetch_or(bit, std::memory_order_release);
+  return PL_OK;
+}
+
+// The codes as [slab][64 rows][head_dim] bytes, slab = (page, layer, head,
+// K or V), read in boxes of `rows` rows under the swizzle of a row's width.
+int codes_map(const pl_kv8* c, int rows, CUtensorMap* m) {
+  typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                               const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                               const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static std::atomic<EncodeFn> encode{nullptr};
+  EncodeFn fn = encode.load(std::memory_order_acquire);
+  if (!fn) {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult res;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &res) !=
+            cudaSuccess ||
+        res != cudaDriverEntryPointSuccess || !p)
+      return PL_ECUDA;
+    fn = reinterpret_cast<EncodeFn>(p);
+    encode.store(fn, std::memory_order_release);
+  }
+  const cuuint64_t hd = static_cast<cuuint64_t>(c->head_dim);
+  const cuuint64_t dims[3] = {
+      hd, PL_KV8_PAGE,
+      static_cast<cuuint64_t>(c->n_pages) * c->n_layers * c->n_kv_heads * 2};
+  const cuuint64_t strides[2] = {hd, hd * PL_KV8_PAGE};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(hd), static_cast<cuuint32_t>(rows), 1u};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c->codes, dims, strides, box, estr,
+         CU_TENSOR_MAP_INTERLEAVE_NONE,
+         c->head_dim == 64 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    std::fprintf(stderr, "pl_attn: cuTensorMapEncodeTiled failed (%d)\n", static_cast<int>(r));
+    return PL_ECUDA;
+  }
+  return PL_OK;
+}
+
 // ------------------------------------------------------------ cache checks
 int check_kv8_shape(const pl_kv8* c) {
   if (!c) return PL_EARG;
@@ -91,7 +147,27 @@ size_t plan_bytes(const pl_kv8* c) {  // src, dst, mark: one int a page each
   return (static_cast<size_t>(c->n_pages) * 4 + 255) / 256 * 256 * 3;
 }
 
-size_t work_bytes(const pl_kv8* c) { return sizeof(pl::Kv8Head) + plan_bytes(c); }
+// One-token attention: two partials a block, then an arrival counter for each
+// entry and head.
+size_t part_bytes(const pl_kv8* c) {
+  return static_cast<size_t>(2) * kMaxBlocks * 32 * (c->head_dim / 4 + 2) * 4;
+}
+size_t arrive_bytes(const pl_kv8* c) {
+  return static_cast<size_t>(pl::kPlanSeqs) * c->n_kv_heads * 4;
+}
+
+size_t work_bytes(const pl_kv8* c) {
+  return sizeof(pl::Kv8Head) + plan_bytes(c) + part_bytes(c) + arrive_bytes(c);
+}
+
+float* work_part(const pl_kv8* c) {
+  return reinterpret_cast<float*>(static_cast<uint8_t*>(c->work) + sizeof(pl::Kv8Head) +
+                                  plan_bytes(c));
+}
+int* work_arrived(const pl_kv8* c) {
+  return reinterpret_cast<int*>(static_cast<uint8_t*>(c->work) + sizeof(pl::Kv8Head) +
+                                plan_bytes(c) + part_bytes(c));
+}
 
 // Every call on a cache: its shape, its memory and the current device.
 int check_kv8(const pl_kv8* c) {
@@ -134,6 +210,8 @@ int check_call(const pl_kv8* c, int layer, int n, const void* d_seqs, const void
       max_tok < 0 || max_tok > c->max_pages * PL_KV8_PAGE || !good_dtype(dtype))
     return PL_EARG;
   if (!d_start && (total != n || max_tok != 1)) return PL_EARG;
+  // tiles of a call are counted in 31 bits
+  if (static_cast<long long>(n) * c->max_pages * c->n_kv_heads * 4 > INT32_MAX) return PL_EARG;
   *none = n == 0 || total == 0 || max_tok == 0;
   if (!*none && !d_seqs) return PL_EARG;
   return PL_OK;
@@ -181,6 +259,22 @@ struct Read {
 template <typename T, int HD, int FMT>
 struct Attend {
   static int run(const pl_kv8* c, const pl::Kv8AttnArgs& a, void* st) {
+    if (a.max_tok == 1) {
+      pl::Kv8DecodeArgs d;
+      d.a = a;
+      d.part = work_part(c);
+      d.arrived = work_arrived(c);
+      CUtensorMap tm;
+      int rc = codes_map(c, pl::DecShape<HD>::kTileRows, &tm);
+      if (rc) return rc;
+      constexpr int smem = static_cast<int>(sizeof(pl::DecSmem<HD>)) + 1024;
+      static_assert(smem <= 227 * 1024, "shared memory of the one-token attention");
+      static std::atomic<unsigned long long> done{0};
+      auto kern = pl::kv8_decode_kernel<T, HD, FMT>;
+      if ((rc = allow_smem(kern, smem, done))) return rc;
+      const int blocks = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
+      return launch(kern, dim3(blocks), pl::kDecThreads, smem, st, true, d, tm);
+    }
     return launch(pl::kv8_attend_plain_kernel<T, HD, FMT>, dim3(a.max_tok, c->n_kv_heads, a.n),
                   pl::kPlainThreads, 0, st, false, a);
   }
@@ -492,7 +586,11 @@ int pl_kv8_status(const pl_kv8* c, void* stream) {
   uint32_t* err = &static_cast<pl::Kv8Head*>(c->work)->err;
   PL_CUDA(cudaMemcpy(&w, err, sizeof(w), cudaMemcpyDeviceToHost));
   if (w) PL_CUDA(cudaMemset(err, 0, sizeof(w)));
-  if (w & (pl::ERR_TIMEOUT_FULL | pl::ERR_TIMEOUT_EMPTY | pl::ERR_TIMEOUT_MMA)) return PL_ETIMEOUT;
+  if (w & (pl::ERR_TIMEOUT_FULL | pl::ERR_TIMEOUT_EMPTY | pl::ERR_TIMEOUT_MMA)) {
+    // a block that gave up has not counted itself
+    PL_CUDA(cudaMemset(work_arrived(c), 0, arrive_bytes(c)));
+    return PL_ETIMEOUT;
+  }
   if (w & pl::ERR_BAD_ARG) return PL_EARG;
   if (w & pl::ERR_NO_PAGES) return PL_ENOMEM;
   return w ? PL_EFAIL : PL_OK;

@@ -132,6 +132,17 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* m, uin
       : "memory");
 }
 
+// Untiled copy of `bytes` (a multiple of 16; both addresses 16-byte aligned)
+// into this CTA's shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes,
+                                          uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+          smem_u32(dst)),
+      "l"(src), "r"(bytes), "r"(smem_u32(bar))
+      : "memory");
+}
+
 // 2-D tiled store of one box from this CTA's shared memory (bulk-group
 // completion: the issuing thread commits and waits on its own groups).
 // Elements of the box outside the tensor are not written.
@@ -196,6 +207,13 @@ __device__ __forceinline__ float2 unpack_half2(uint32_t h) {
       : "=f"(f.x), "=f"(f.y)
       : "r"(h));
   return f;
+}
+
+// Split an FP32 pair into FP16 high parts and FP16 residuals.
+__device__ __forceinline__ void split_hi_lo(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_half2(a, b);
+  const float2 h = unpack_half2(hi);
+  lo = pack_half2(a - h.x, b - h.y);
 }
 
 // max of three floats in one instruction.
