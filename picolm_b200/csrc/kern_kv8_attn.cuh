@@ -156,36 +156,45 @@ __global__ void __launch_bounds__(kPlainThreads) kv8_attend_plain_kernel(
 // memory by the warp where the run starts; runs over several blocks leave
 // one partial a block in the workspace, and the block that finishes a run's
 // last partial merges them, in the order of the blocks.
-constexpr int kDecWarps = 8;
-constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecTileBytes = 4096;  // of K, and of V
 constexpr float kWeightScale = 16384.f;
 constexpr float kMinRef = 1e-30f;
 
-template <int HD>
-struct DecShape {
-  static constexpr int kTileRows = kDecTileBytes / HD;    // 64 or 32
+template <int W, int TR, int NS, int HD>
+struct DecShapeT {
+  static constexpr int kWarps = W;
+  static constexpr int kThreads = W * 32;
+  static constexpr int kTileRows = TR;
+  static constexpr int kTileBytes = TR * HD;              // of K, and of V
   static constexpr int kTilesPerPage = kPage / kTileRows;
   static constexpr int kBlocks = kTileRows / kBlock;      // scales in a tile
-  static constexpr int kStages = HD == 64 ? 3 : 2;
-  static constexpr int kPartFloats = 32 * (HD / 4 + 2);   // a partial: lane-wise m, l, o
+  static constexpr int kStages = NS;
+  static constexpr int kPartFloats = 32 * (HD / 4) + 16;  // a partial: o lane-wise, then m, l
 };
+
+template <int HD>
+struct DecShape : DecShapeT<8, 64, 3, 64> {};
+template <>
+struct DecShape<128> : DecShapeT<8, 32, 2, 128> {};
 
 template <int HD>
 struct DecSmem {
   using Sh = DecShape<HD>;
-  uint8_t ring[kDecWarps][Sh::kStages][2][kDecTileBytes];  // 1024-byte aligned
-  float scales[kDecWarps][Sh::kStages][2][kBlocksPerPage];
-  float part[kDecWarps][Sh::kPartFloats];
-  float2 cs[kDecWarps][HD / 2];
-  uint64_t full[kDecWarps][Sh::kStages];
-  int prefix[kPlanSeqs + 1];
-  int warp_sum[kDecWarps];
+  uint8_t ring[Sh::kWarps][Sh::kStages][2][Sh::kTileBytes];  // 1024-byte aligned
+  float scales[Sh::kWarps][Sh::kStages][2][kBlocksPerPage];
+  float part[Sh::kWarps][Sh::kPartFloats];
+  float2 cs[Sh::kWarps][HD / 2];
+  double half_turns[HD / 2];
+  uint64_t full[Sh::kWarps][Sh::kStages];
+  int prefix[kPlanSeqs + 1], slot[kPlanSeqs], len[kPlanSeqs];
+  int warp_sum[Sh::kWarps];
+  int ended[4];   // of the run that an earlier block began: run, first, last tile, warp that has it
   int finish[2];
 };
 
 struct Kv8DecodeArgs {
   Kv8AttnArgs a;
+  const void *k, *v;  // one row an entry, appended first (APPEND)
+  long long k_stride, v_stride;
   float* part;    // [2 * blocks][kPartFloats]
   int* arrived;   // [entries * kv heads], zero at rest
 };
@@ -217,44 +226,60 @@ __device__ __forceinline__ void store4(__nv_bfloat16* p, const float (&x)[4]) {
                                             *reinterpret_cast<const uint32_t*>(&b));
 }
 
-// Elements [e, e + 4) of a head row, rotated (e a multiple of 4).
-template <typename T>
-__device__ __forceinline__ void load_rotated4(const T* x, int e, const pl_rope& r, const float2* cs,
-                                              float (&y)[4]) {
-  load4(x + e, y);
-  if (e >= r.dim) return;
-  const int half = r.dim >> 1;
-  if (r.type == PL_ROPE_LLAMA) {
+// A row's elements 16j + 4c .. + 3, and those they rotate with: all loads
+// of a row are issued before one is used.
+template <typename T, int HD>
+struct QRow {
+  float y[HD / 16][4], z[HD / 16][4];
+  __device__ __forceinline__ void load(const T* x, int c, const pl_rope& r) {
+    const int half = r.dim >> 1;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (e + 2 * j >= r.dim) break;
-      const float2 c = cs[(e >> 1) + j];
-      const float a = y[2 * j], b = y[2 * j + 1];
-      y[2 * j] = a * c.x - b * c.y;
-      y[2 * j + 1] = a * c.y + b * c.x;
-    }
-  } else if (half % 4 == 0) {
-    const bool first = e < half;
-    float z[4];
-    load4(x + (first ? e + half : e - half), z);
+    for (int j = 0; j < HD / 16; ++j) load4(x + 16 * j + 4 * c, y[j]);
+    if (r.type == PL_ROPE_QWEN) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 c = cs[(first ? e : e - half) + j];
-      y[j] = first ? y[j] * c.x - z[j] * c.y : z[j] * c.y + y[j] * c.x;
-    }
-  } else {
+      for (int j = 0; j < HD / 16; ++j) {
+        const int e = 16 * j + 4 * c;
+        if (half % 4 == 0) {
+          const int o = e < half ? e + half : e < r.dim ? e - half : e;
+          load4(x + o, z[j]);
+        } else {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int d = e + j;
-      if (d >= r.dim) break;
-      if (d < half) {
-        y[j] = y[j] * cs[d].x - to_f32(x[d + half]) * cs[d].y;
-      } else {
-        y[j] = to_f32(x[d - half]) * cs[d - half].y + y[j] * cs[d - half].x;
+          for (int k = 0; k < 4; ++k) {
+            const int d = e + k;
+            z[j][k] = to_f32(x[d < half ? d + half : d < r.dim ? d - half : d]);
+          }
+        }
       }
     }
   }
-}
+  // cs: cosine and sine of the pairs
+  __device__ __forceinline__ void rotate(int c, const pl_rope& r, const float2* cs) {
+    const int half = r.dim >> 1;
+#pragma unroll
+    for (int j = 0; j < HD / 16; ++j) {
+      const int e = 16 * j + 4 * c;
+      if (r.type == PL_ROPE_LLAMA) {
+#pragma unroll
+        for (int k = 0; k < 4; k += 2)
+          if (e + k < r.dim) {
+            const float2 f = cs[(e + k) >> 1];
+            const float a = y[j][k], b = y[j][k + 1];
+            y[j][k] = a * f.x - b * f.y;
+            y[j][k + 1] = a * f.y + b * f.x;
+          }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int d = e + k;
+          if (d < r.dim) {
+            const float2 f = cs[d < half ? d : d - half];
+            y[j][k] = d < half ? y[j][k] * f.x - z[j][k] * f.y : z[j][k] * f.y + y[j][k] * f.x;
+          }
+        }
+      }
+    }
+  }
+};
 
 // Codes as FP16 pairs.  int8: the byte with its sign bit flipped below a
 // 0x64 is 1024 + 128 + code in FP16; e4m3 converts in hardware.
@@ -308,7 +333,8 @@ struct DecWork {
 };
 
 // Running state of a segment: row g = lane / 4 of the A operand is query
-// head g of the KV head, this thread holds its dims 16ch + 4(lane % 4) ..
+// head g of the KV head; of each 16-byte chunk ch this thread holds the dims
+// 16ch + 4(lane % 4) + {0, 2, 1, 3}, in o[4ch ..] (even and odd n-tile).
 template <int HD>
 struct DecState {
   float m, l, o[HD / 4];
@@ -331,17 +357,32 @@ struct DecState {
     m = mx;
   }
   __device__ __forceinline__ void save(float* p, int lane) const {
-    p[lane] = m;
-    p[32 + lane] = l;
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) p[(2 + i) * 32 + lane] = o[i];
+    for (int i = 0; i < HD / 4; ++i) p[i * 32 + lane] = o[i];
+    if ((lane & 3) == 0) {
+      p[8 * HD + (lane >> 2)] = m;
+      p[8 * HD + 8 + (lane >> 2)] = l;
+    }
   }
   __device__ __forceinline__ void fold_from(const float* p, int lane) {
     float o2[HD / 4];
-    const float m2 = p[lane], l2 = p[32 + lane];
+    const float m2 = p[8 * HD + (lane >> 2)], l2 = p[8 * HD + 8 + (lane >> 2)];
 #pragma unroll
-    for (int i = 0; i < HD / 4; ++i) o2[i] = p[(2 + i) * 32 + lane];
+    for (int i = 0; i < HD / 4; ++i) o2[i] = p[i * 32 + lane];
     fold(m2, l2, o2);
+  }
+  // Two partials from global memory (the second if `two`), loaded at once.
+  __device__ __forceinline__ void fold_two(const float* p, const float* q, bool two, int lane) {
+    float po[HD / 4], qo[HD / 4];
+    const float pm = __ldcg(p + 8 * HD + (lane >> 2)), pl_ = __ldcg(p + 8 * HD + 8 + (lane >> 2));
+    const float qm = __ldcg(q + 8 * HD + (lane >> 2)), ql = __ldcg(q + 8 * HD + 8 + (lane >> 2));
+#pragma unroll
+    for (int i = 0; i < HD / 4; ++i) {
+      po[i] = __ldcg(p + i * 32 + lane);
+      qo[i] = __ldcg(q + i * 32 + lane);
+    }
+    fold(pm, pl_, po);
+    if (two) fold(qm, ql, qo);
   }
   template <typename T>
   __device__ __forceinline__ void write(T* out, int lane, int group) const {
@@ -350,18 +391,80 @@ struct DecState {
     const float inv = 1.0f / l;
 #pragma unroll
     for (int ch = 0; ch < HD / 16; ++ch) {
-      const float x[4] = {o[4 * ch] * inv, o[4 * ch + 1] * inv, o[4 * ch + 2] * inv,
+      const float x[4] = {o[4 * ch] * inv, o[4 * ch + 2] * inv, o[4 * ch + 1] * inv,
                           o[4 * ch + 3] * inv};
       store4(out + g * HD + 16 * ch + 4 * c, x);
     }
   }
 };
 
-template <typename T, int HD, int FMT>
-__global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
+// ---- a warp appends a row to a tile it holds
+template <int FMT>
+__device__ __forceinline__ uint32_t encode1(float x) {
+  if constexpr (FMT == PL_KV8_INT8)
+    return static_cast<uint32_t>(__float2int_rn(fminf(fmaxf(x, -127.f), 127.f))) & 0xffu;
+  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+
+// The quantisation of kv8_append_kernel for one new row `r` (of k or v) of a
+// tile in shared memory, there and in global memory.  x: this lane's HD / 32
+// consecutive elements, rotated; tile, gtile: the tile's row 0; block: first
+// row of r's block; s_scale, g_scale: the block's scale.
+template <int HD, int FMT>
+__device__ __forceinline__ void append_row(const float (&x)[HD / 32], int lane, int r, int block,
+                                           uint32_t tile, uint8_t* gtile, float* s_scale,
+                                           float* g_scale) {
+  constexpr int E = HD / 32;
+  uint32_t top = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) top = max(top, __float_as_uint(fabsf(x[j])));
+  top = __reduce_max_sync(0xffffffffu, top);
+  const uint32_t old_bits = r > block ? __float_as_uint(*s_scale) : 0u;
+  float s = __fdiv_rn(__uint_as_float(top), code_top<FMT>());
+  if (top >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
+  s = __uint_as_float(max(__float_as_uint(s), old_bits));
+  const float by = s > 0.f ? s : 1.f;
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) {
+    *s_scale = s;
+    *g_scale = s;
+  }
+  uint32_t code = 0;
+#pragma unroll
+  for (int j = 0; j < E; ++j) code |= encode1<FMT>(__fdiv_rn(x[j], by)) << (8 * j);
+  const int el = lane * E;
+  const uint32_t at = tile + tile_off<HD>(r, el >> 4) + (el & 15);
+  if constexpr (E == 2) {
+    asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(static_cast<uint16_t>(code)) : "memory");
+    *reinterpret_cast<uint16_t*>(gtile + r * HD + el) = static_cast<uint16_t>(code);
+  } else {
+    asm volatile("st.shared.u32 [%0], %1;" ::"r"(at), "r"(code) : "memory");
+    *reinterpret_cast<uint32_t*>(gtile + r * HD + el) = code;
+  }
+  if (__float_as_uint(s) != old_bits && r > block) {  // the scale has grown
+    const float ratio = s > 0.f ? __fdiv_rn(__uint_as_float(old_bits), s) : 1.f;
+    for (int o = lane * 8; o < (r - block) * HD; o += 256) {
+      const int row = block + o / HD, e = o % HD;
+      const uint32_t p = tile + tile_off<HD>(row, e >> 4) + (e & 15);
+      uint2 c;
+      asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(c.x), "=r"(c.y) : "r"(p) : "memory");
+      float y[8];
+      decode8<FMT>(c, y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = __fmul_rn(y[j], ratio);
+      c = encode8<FMT>(y);
+      asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(p), "r"(c.x), "r"(c.y) : "memory");
+      *reinterpret_cast<uint2*>(gtile + row * HD + e) = c;
+    }
+  }
+  __syncwarp();
+}
+
+template <typename T, int HD, int FMT, bool APPEND>
+__global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
     const __grid_constant__ Kv8DecodeArgs da, const __grid_constant__ CUtensorMap tm) {
   using Sh = DecShape<HD>;
-  constexpr int NS = Sh::kStages, TR = Sh::kTileRows;
+  constexpr int W = Sh::kWarps, NS = Sh::kStages, TR = Sh::kTileRows;
   extern __shared__ uint8_t smem_raw[];
   DecSmem<HD>& sm = *reinterpret_cast<DecSmem<HD>*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -369,6 +472,8 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
   const int heads = a.g.n_kv_heads, G = a.group;
+  // the frequencies to shared memory: lanes of a warp want different ones
+  if (tid < HD / 2) sm.half_turns[tid] = a.rope.half_turns[tid];
   if (lane == 0) {
     for (int s = 0; s < NS; ++s) mbar_init(&sm.full[warp][s], 1);
     fence_mbar_init();
@@ -376,19 +481,23 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
   }
   __syncwarp();
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // ---- tiles of every entry, scanned
   {
-    const int per = (a.n + kDecThreads - 1) / kDecThreads, i0 = tid * per;
+    const int per = (a.n + Sh::kThreads - 1) / Sh::kThreads, i0 = tid * per;
     int mine = 0;
     bool bad = false;
     for (int i = i0; i < min(a.n, i0 + per); ++i) {
       Kv8Entry e;
-      const bool ok = kv8_entry(a.g, i, a.total, 1, a.seqs, a.start, e);
+      bool ok = kv8_entry(a.g, i, a.total, 1, a.seqs, a.start, e);
+      if (APPEND) ok = ok && e.len > 0;
       bad |= !ok;
       const int rows = ok && e.n_tok ? e.len : 0;
       const int tiles = (rows + TR - 1) / TR * heads;
       sm.prefix[i] = tiles;
+      sm.slot[i] = e.slot;
+      sm.len[i] = rows;
       mine += tiles;
       // nothing to attend: zeros
       if (ok && e.n_tok && e.len == 0 && blockIdx.x == 0)
@@ -406,7 +515,7 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
     __syncthreads();
     int base = 0, total = 0;
 #pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       base += w < warp ? sm.warp_sum[w] : 0;
       total += sm.warp_sum[w];
     }
@@ -419,164 +528,202 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
     if (tid == 0) {
       sm.prefix[a.n] = total;
       sm.finish[0] = sm.finish[1] = -1;
+      sm.ended[0] = -1;
     }
     __syncthreads();
   }
   const int total = sm.prefix[a.n];
-  const DecWork<HD> work{sm.prefix, a.n, heads, total, min(static_cast<int>(gridDim.x), total)};
+  // at least a tile for each warp of a block: fewer blocks share a run then
+  const DecWork<HD> work{sm.prefix, a.n, heads, total,
+                         min(static_cast<int>(gridDim.x), (total + W - 1) / W)};
   const int blk = blockIdx.x;
   if (blk >= work.blocks) return;
   const int b0 = work.begin(blk), b1 = work.begin(blk + 1), span = b1 - b0;
-  const int x0 = b0 + static_cast<int>(static_cast<long long>(warp) * span / kDecWarps);
-  const int x1 = b0 + static_cast<int>(static_cast<long long>(warp + 1) * span / kDecWarps);
+  const int x0 = b0 + warp * span / W, x1 = b0 + (warp + 1) * span / W;
 
-  // ---- this warp's tiles: 32 at a time, tile x0 + 32k + lane in this lane
-  int t_run = 0, t_row = 0, t_slab = 0, t_len = 0, t_base = x0 - 32;
-  auto fetch_tiles = [&](int base) {
+  // ---- this warp's tiles: 32 at a time, tile t_base + lane in this lane
+  int t_run = 0, t_row = 0, t_slab = 0, t_base = x0;
+  auto find_tile = [&](int base) -> int {  // the page, not yet checked
     t_base = base;
     const int x = base + lane;
-    if (x < x1) {
-      const int i = work.entry_of(x);
-      const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
-      const int rem = x - sm.prefix[i], h = rem / tiles, t = rem - h * tiles;
-      const int slot = a.seqs[i];
-      int page = a.g.table[static_cast<long long>(slot) * a.g.max_pages + t / Sh::kTilesPerPage];
-      t_len = a.g.lens[slot];
-      if (page < 0 || page >= a.g.n_pages) {
-        atomicOr(&a.g.head->err, ERR_BAD_ARG);
-        page = 0;
-      }
-      t_run = i * heads + h;
-      t_row = t * TR;
-      t_slab = static_cast<int>(a.g.slab(page, h, 0));
+    if (x >= x1) return 0;
+    const int i = work.entry_of(x);
+    const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
+    const int rem = x - sm.prefix[i], h = rem / tiles, t = rem - h * tiles;
+    t_run = i * heads + h;
+    t_row = t * TR;
+    return a.g.table[static_cast<long long>(sm.slot[i]) * a.g.max_pages + t / Sh::kTilesPerPage];
+  };
+  auto place_tile = [&](int page) {
+    if (page < 0 || page >= a.g.n_pages) {
+      atomicOr(&a.g.head->err, ERR_BAD_ARG);
+      page = 0;
+    }
+    t_slab = static_cast<int>(a.g.slab(page, t_run % heads, 0));
+  };
+  auto issue = [&](int x) {
+    const int slab = __shfl_sync(0xffffffffu, t_slab, x - t_base);
+    const int row = __shfl_sync(0xffffffffu, t_row, x - t_base);
+    if (lane == 0) {
+      const int s = (x - x0) % NS;
+      uint64_t* bar = &sm.full[warp][s];
+      mbar_arrive_expect_tx(bar, 2 * Sh::kTileBytes + 2 * kBlocksPerPage * 4);
+      tma_load_3d(sm.ring[warp][s][0], &tm, bar, 0, row % kPage, slab);
+      tma_load_3d(sm.ring[warp][s][1], &tm, bar, 0, row % kPage, slab + 1);
+      bulk_load(sm.scales[warp][s], a.g.scales + static_cast<long long>(slab) * kBlocksPerPage,
+                2 * kBlocksPerPage * 4, bar);
     }
   };
-  auto issue = [&](int x, int slab, int row) {  // lane 0
-    const int s = (x - x0) % NS;
-    uint64_t* bar = &sm.full[warp][s];
-    mbar_arrive_expect_tx(bar, 2 * kDecTileBytes + 2 * kBlocksPerPage * 4);
-    tma_load_3d(sm.ring[warp][s][0], &tm, bar, 0, row % kPage, slab);
-    tma_load_3d(sm.ring[warp][s][1], &tm, bar, 0, row % kPage, slab + 1);
-    bulk_load(sm.scales[warp][s], a.g.scales + static_cast<long long>(slab) * kBlocksPerPage,
-              2 * kBlocksPerPage * 4, bar);
+  // the query rows of a run, as they are in memory
+  QRow<T, HD> q;
+  auto load_q = [&](int run) {
+    const int i = run / heads, h = run - i * heads, tok = a.start ? a.start[i] : i;
+    q.load(static_cast<const T*>(a.q) + tok * a.q_stride + (h * G + min(g, G - 1)) * HD, c, a.rope);
   };
   bool ok = true;
   int issued = x0;
-  if (x0 < x1) fetch_tiles(x0);
-  for (; issued < x1 && issued < x0 + NS; ++issued) {
-    const int slab = __shfl_sync(0xffffffffu, t_slab, issued - t_base);
-    const int row = __shfl_sync(0xffffffffu, t_row, issued - t_base);
-    if (lane == 0) issue(issued, slab, row);
+  if (x0 < x1) {
+    const int page = find_tile(x0);
+    load_q(__shfl_sync(0xffffffffu, t_run, 0));
+    place_tile(page);
+    for (; issued < x1 && issued < x0 + NS; ++issued) issue(issued);
   }
 
   uint32_t qa[HD / 16][4];
   DecState<HD> st;
   st.clear();
-  // This block's partial of a run over several blocks (kind 0: the run
-  // started before the block, 1: in it); the last block to leave one is to
-  // merge them.
-  auto publish = [&](int r, int first, int last, int kind) {
-    st.save(da.part + static_cast<long long>(2 * blk + kind) * Sh::kPartFloats, lane);
-    __threadfence();
-    __syncwarp();
-    if (lane == 0) {
-      const int parts = work.block_of(last) - work.block_of(first) + 1;
-      if (atomicAdd(&da.arrived[r], 1) == parts - 1) {
-        da.arrived[r] = 0;
-        __threadfence();
-        sm.finish[kind] = r;
-      }
-    }
-    __syncwarp();
-  };
   float ref = kMinRef, q_scale = 0.f;
-  int run = -1, run_first = 0, run_last = 0;  // the current run and its tiles
+  int run = -1, run_first = 0, run_last = 0, len = 0;  // the current run and its tiles
   const uint32_t ring = smem_u32(sm.ring[warp]);
-  // tile fields of the consumed tile live one batch behind the issued ones
-  int c_run = t_run, c_row = t_row, c_len = t_len, c_base = t_base;
+  // tiles are consumed a few behind the issued ones: a batch of their own
+  int c_run = t_run, c_row = t_row, c_slab = t_slab, c_base = t_base;
   for (int x = x0; x < x1 && ok; ++x) {
     if (x - c_base >= 32) {
-      c_run = t_run, c_row = t_row, c_len = t_len, c_base = t_base;
+      c_run = t_run, c_row = t_row, c_slab = t_slab, c_base = t_base;
     }
     const int x_run = __shfl_sync(0xffffffffu, c_run, x - c_base);
     const int row0 = __shfl_sync(0xffffffffu, c_row, x - c_base);
-    const int len = __shfl_sync(0xffffffffu, c_len, x - c_base);
     const int i = x_run / heads, h = x_run - i * heads;
     if (x_run != run) {
-      // ---- a new run: its query rows
+      // ---- a new run: its query rows, rotated, scaled and split
       run = x_run;
       const int tiles = (sm.prefix[i + 1] - sm.prefix[i]) / heads;
       run_first = sm.prefix[i] + h * tiles;
       run_last = run_first + tiles - 1;
-      const int tok = a.start ? a.start[i] : i;
+      len = sm.len[i];
+      if (x != x0) load_q(run);
       for (int p = lane; p < a.rope.dim >> 1; p += 32)
-        sm.cs[warp][p] = rope_cs_fast(a.rope, p, len - 1);
+        sm.cs[warp][p] = rope_cs_fast(sm.half_turns[p], a.rope.gain, len - 1);
       __syncwarp();
-      const T* q = static_cast<const T*>(a.q) + tok * a.q_stride + (h * G + min(g, G - 1)) * HD;
-      float y[HD / 16][4], top = 0.f;
-#pragma unroll
-      for (int j = 0; j < HD / 16; ++j) {
-        load_rotated4(q, 16 * j + 4 * c, a.rope, sm.cs[warp], y[j]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(y[j][e]));
-      }
+      q.rotate(c, a.rope, sm.cs[warp]);
       __syncwarp();
+      float top = 0.f;
+#pragma unroll
+      for (int j = 0; j < HD / 16; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) top = fmaxf(top, fabsf(q.y[j][e]));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^-e with 2^e <= top < 2^(e+1), for normal finite tops
       const uint32_t ex = __float_as_uint(top) >> 23;
       const bool norm = ex > 1 && ex < 253;
-      const float down = norm ? __uint_as_float((254u - ex) << 23) : 1.f;
+      const float down = g >= G ? 0.f : norm ? __uint_as_float((254u - ex) << 23) : 1.f;
       q_scale = (norm ? __uint_as_float(ex << 23) : 1.f) * a.score_scale;
 #pragma unroll
       for (int j = 0; j < HD / 16; ++j)
 #pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const float u = g < G ? y[j][2 * hf] * down : 0.f;
-          const float v = g < G ? y[j][2 * hf + 1] * down : 0.f;
-          split_hi_lo(u, v, qa[j][2 * hf], qa[j][2 * hf + 1]);
-        }
+        for (int hf = 0; hf < 2; ++hf)
+          split_hi_lo(q.y[j][2 * hf] * down, q.y[j][2 * hf + 1] * down, qa[j][2 * hf],
+                      qa[j][2 * hf + 1]);
       st.clear();
       ref = kMinRef;
     }
     const int s = (x - x0) % NS;
+    const uint32_t kt = ring + s * 2 * Sh::kTileBytes, vt = kt + Sh::kTileBytes;
+    float* sk = sm.scales[warp][s][0] + row0 % kPage / kBlock;
+    float* sv = sm.scales[warp][s][1] + row0 % kPage / kBlock;
+    const int seen = len - row0;  // rows of the tile, at least 1
+    // ---- the entry's new row belongs to this tile: fetched before the wait
+    constexpr int E = HD / 32;
+    float kx[E], vx[E];
+    const bool appends = APPEND && seen <= TR;
+    if (appends) {
+      for (int p = lane; p < a.rope.dim >> 1; p += 32)
+        sm.cs[warp][p] = rope_cs(sm.half_turns[p], a.rope.gain, len - 1);
+      const T* k = static_cast<const T*>(da.k) + i * da.k_stride + h * HD;
+      const T* v = static_cast<const T*>(da.v) + i * da.v_stride + h * HD;
+      const int half = a.rope.dim >> 1;
+      __syncwarp();
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const int d = lane * E + j;
+        const float own = to_f32(k[d]);
+        vx[j] = to_f32(v[d]);
+        kx[j] = own;
+        if (d < a.rope.dim) {
+          const bool llama = a.rope.type == PL_ROPE_LLAMA;
+          const bool first = llama ? !(d & 1) : d < half;
+          const float other = to_f32(k[llama ? d ^ 1 : first ? d + half : d - half]);
+          const float2 f = sm.cs[warp][llama ? d >> 1 : first ? d : d - half];
+          kx[j] = first ? __fsub_rn(__fmul_rn(own, f.x), __fmul_rn(other, f.y))
+                        : __fadd_rn(__fmul_rn(other, f.y), __fmul_rn(own, f.x));
+        }
+      }
+    }
     if (!mbar_wait_bounded(&sm.full[warp][s], ((x - x0) / NS) & 1)) {
       if (lane == 0) atomicOr(&a.g.head->err, ERR_TIMEOUT_FULL);
       ok = false;
       break;
     }
-    const uint32_t kt = ring + s * 2 * kDecTileBytes, vt = kt + kDecTileBytes;
-    const float* sk = sm.scales[warp][s][0] + row0 % kPage / kBlock;
-    const float* sv = sm.scales[warp][s][1] + row0 % kPage / kBlock;
+    if (appends) {
+      const int r = seen - 1, block = r / kBlock * kBlock;
+      const long long slab = __shfl_sync(0xffffffffu, c_slab, x - c_base);
+      const int b = (row0 % kPage + block) / kBlock;
+      uint8_t* gt = a.g.codes + (slab * kPage + row0 % kPage) * HD;
+      append_row<HD, FMT>(kx, lane, r, block, kt, gt, &sm.scales[warp][s][0][b],
+                          a.g.scales + slab * kBlocksPerPage + b);
+      append_row<HD, FMT>(vx, lane, r, block, vt, gt + kPage * HD, &sm.scales[warp][s][1][b],
+                          a.g.scales + (slab + 1) * kBlocksPerPage + b);
+    }
     // ---- S = Q K^T
-    float sc[TR / 8][4];
+    float2 sc[TR / 8];  // this thread's columns 8nt + 2c, + 1 of row g
+    float mt = -INFINITY;
 #pragma unroll
     for (int nt = 0; nt < TR / 8; ++nt) {
-      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      float acc[4];
 #pragma unroll
       for (int q4 = 0; q4 < HD / 64; ++q4) {
         uint32_t w[4];
         ldmatrix_x4(kt + tile_off<HD>(nt * 8 + (lane & 7), 4 * q4 + (lane >> 3)), w[0], w[1], w[2],
                     w[3]);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          mma_16816(sc[nt], qa[4 * q4 + j], codes_half2<FMT, 0x10>(w[j]),
-                    codes_half2<FMT, 0x32>(w[j]));
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t b0 = codes_half2<FMT, 0x10>(w[j]), b1 = codes_half2<FMT, 0x32>(w[j]);
+          if (q4 == 0 && j == 0) mma_16816_zero(acc, qa[0], b0, b1);
+          else mma_16816(acc, qa[4 * q4 + j], b0, b1);
+        }
       }
-    }
-    const bool tail = row0 + TR > len;
-    float mt = -INFINITY;
-#pragma unroll
-    for (int nt = 0; nt < TR / 8; ++nt) {
       const float by = q_scale * sk[nt / 2];
+      sc[nt] = mul2(add2(make_float2(acc[0], acc[1]), make_float2(acc[2], acc[3])),
+                    make_float2(by, by));
+    }
+    if (seen < TR) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float v = (sc[nt][e] + sc[nt][2 + e]) * by;
-        if (tail && row0 + nt * 8 + 2 * c + e >= len) v = -INFINITY;
-        sc[nt][e] = v;
-        mt = fmaxf(mt, v);
+      for (int nt = 0; nt < TR / 8; ++nt) {
+        if (nt * 8 + 2 * c >= seen) sc[nt].x = -INFINITY;
+        if (nt * 8 + 2 * c + 1 >= seen) sc[nt].y = -INFINITY;
+      }
+      if constexpr (FMT == PL_KV8_E4M3) {
+        // rows past the end weigh 0, but their bytes may be NaN codes
+        for (int o = seen * HD + lane * 16; o < TR * HD; o += 512)
+          asm volatile("st.shared.v4.u32 [%0], {%1, %1, %1, %1};" ::"r"(vt + o), "r"(0) : "memory");
+        __syncwarp();
       }
     }
+    // generic writes to the stage come before it is filled again
+    if (appends || (FMT == PL_KV8_E4M3 && seen < TR)) fence_proxy_async_smem();
+#pragma unroll
+    for (int nt = 0; nt < TR / 8; ++nt) mt = max3(mt, sc[nt].x, sc[nt].y);
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
     mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
     const float m_new = fmaxf(st.m, mt);
@@ -584,65 +731,61 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
     float top = sv[0];
 #pragma unroll
     for (int b = 1; b < Sh::kBlocks; ++b)
-      if (row0 + b * kBlock < len) top = fmaxf(top, sv[b]);
+      if (b * kBlock < seen) top = fmaxf(top, sv[b]);
     const float ref_new = fmaxf(ref, top);
     const float keep = alpha * (ref / ref_new), lift = kWeightScale / ref_new;
     ref = ref_new;
     st.m = m_new;
-    st.l *= alpha;
-    // ---- O = O * keep + P V
-    float ot[HD / 8][4];
-#pragma unroll
-    for (int j = 0; j < HD / 8; ++j) ot[j][0] = ot[j][1] = ot[j][2] = ot[j][3] = 0.f;
+    // ---- the weights, as A fragments
+    uint32_t pa[Sh::kBlocks][4];
+    float2 sum = make_float2(0.f, 0.f);
+    const float2 nm = make_float2(-m_new, -m_new);
 #pragma unroll
     for (int b = 0; b < Sh::kBlocks; ++b) {
-      if (row0 + b * kBlock >= len) break;
-      const float by = sv[b] * lift;
-      uint32_t pa[4];
+      const float by = b * kBlock < seen ? sv[b] * lift : 0.f;
 #pragma unroll
       for (int hf = 0; hf < 2; ++hf) {
-        const float p0 = ex2(sc[2 * b + hf][0] - m_new), p1 = ex2(sc[2 * b + hf][1] - m_new);
-        st.l += p0 + p1;
-        split_hi_lo(p0 * by, p1 * by, pa[2 * hf], pa[2 * hf + 1]);
+        const float2 x = add2(sc[2 * b + hf], nm);
+        const float2 p = make_float2(ex2(x.x), ex2(x.y));
+        sum = add2(sum, p);
+        const float2 w = mul2(p, make_float2(by, by));
+        split_hi_lo(w.x, w.y, pa[b][2 * hf], pa[b][2 * hf + 1]);
       }
-      // rows past the end weigh 0, but their bytes may be NaN codes
-      uint32_t seen0 = 0xffffffffu, seen1 = 0xffffffffu;
-      if (tail) {
-        const int r = row0 + b * kBlock + 2 * c;
-        seen0 = (r < len ? 0xffffu : 0u) | (r + 1 < len ? 0xffff0000u : 0u);
-        seen1 = (r + 8 < len ? 0xffffu : 0u) | (r + 9 < len ? 0xffff0000u : 0u);
-      }
+    }
+    st.l = fmaf(st.l, alpha, sum.x + sum.y);
+    // ---- O = O * keep + P V, 32 dims at a time
 #pragma unroll
-      for (int ch = 0; ch < HD / 16; ch += 2) {
+    for (int ch = 0; ch < HD / 16; ch += 2) {
+      float ot[4][4];  // even and odd dims of chunk ch, then of ch + 1
+#pragma unroll
+      for (int b = 0; b < Sh::kBlocks; ++b) {
         uint32_t w[4];  // (rows 0-7, 8-15) of chunk ch, then of ch + 1
         ldmatrix_x4_trans(vt + tile_off<HD>(b * kBlock + ((lane >> 3) & 1) * 8 + (lane & 7),
                                             ch + (lane >> 4)),
                           w[0], w[1], w[2], w[3]);
-        w[0] &= seen0, w[1] &= seen1, w[2] &= seen0, w[3] &= seen1;
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          mma_16816(ot[2 * (ch + k)], pa, codes_half2<FMT, 0x20>(w[2 * k]),
-                    codes_half2<FMT, 0x20>(w[2 * k + 1]));
-          mma_16816(ot[2 * (ch + k) + 1], pa, codes_half2<FMT, 0x31>(w[2 * k]),
-                    codes_half2<FMT, 0x31>(w[2 * k + 1]));
+        for (int k = 0; k < 4; ++k) {
+          const uint32_t b0 = k & 1 ? codes_half2<FMT, 0x31>(w[k & 2]) : codes_half2<FMT, 0x20>(w[k & 2]);
+          const uint32_t b1 =
+              k & 1 ? codes_half2<FMT, 0x31>(w[(k & 2) + 1]) : codes_half2<FMT, 0x20>(w[(k & 2) + 1]);
+          if (b == 0) mma_16816_zero(ot[k], pa[b], b0, b1);
+          else mma_16816(ot[k], pa[b], b0, b1);
         }
       }
-    }
-    // n-tiles 2ch, 2ch+1 hold the dims 16ch + 4c + {0, 2} and {1, 3}
 #pragma unroll
-    for (int ch = 0; ch < HD / 16; ++ch)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float* t = ot[2 * ch + (e & 1)];
-        st.o[4 * ch + e] = fmaf(st.o[4 * ch + e], keep, t[e >> 1] + t[2 + (e >> 1)]);
+      for (int k = 0; k < 4; ++k) {
+        float* o = &st.o[4 * ch + 2 * k];
+        const float2 t = fma2(make_float2(o[0], o[1]), make_float2(keep, keep),
+                              add2(make_float2(ot[k][0], ot[k][1]), make_float2(ot[k][2], ot[k][3])));
+        o[0] = t.x;
+        o[1] = t.y;
       }
+    }
     // ---- the stage is free: the next tile
     __syncwarp();
     if (issued < x1) {
-      if (issued - t_base >= 32) fetch_tiles(issued);
-      const int slab = __shfl_sync(0xffffffffu, t_slab, issued - t_base);
-      const int row = __shfl_sync(0xffffffffu, t_row, issued - t_base);
-      if (lane == 0) issue(issued, slab, row);
+      if (issued - t_base >= 32) place_tile(find_tile(issued));
+      issue(issued);
       ++issued;
     }
     // ---- the segment's end
@@ -658,7 +801,14 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
         const int tok = a.start ? a.start[i] : i;
         st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
       } else if (x != x1 - 1) {
-        publish(run, run_first, run_last, 0);  // the end of an earlier block's run
+        // the end of an earlier block's run, with more to do: left for later
+        st.save(sm.part[warp], lane);
+        if (lane == 0) {
+          sm.ended[0] = run;
+          sm.ended[1] = run_first;
+          sm.ended[2] = run_last;
+          sm.ended[3] = warp;
+        }
       }
     }
   }
@@ -667,27 +817,61 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
     mbar_wait_bounded(&sm.full[warp][(x - x0) % NS], ((x - x0) / NS) & 1);
   __syncthreads();
 
+  auto write_run = [&](int r) {
+    const int i = r / heads, h = r - i * heads, tok = a.start ? a.start[i] : i;
+    st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
+  };
+  // The p-th block's partial of the run with first tile `first` in block f0.
+  auto partial = [&](int f0, int p, int first) {
+    const int slot = 2 * (f0 + p) + (first >= work.begin(f0 + p) ? 1 : 0);
+    return da.part + static_cast<long long>(slot) * Sh::kPartFloats;
+  };
+  // `st` is this block's partial of a run over several blocks (kind 0: one
+  // that started before the block, 1: in it).  The block that leaves the
+  // last one merges them in the order of the blocks: a few at once here,
+  // more of them with all warps below.
+  auto publish = [&](int r, int first, int last, int kind) {
+    st.save(da.part + static_cast<long long>(2 * blk + kind) * Sh::kPartFloats, lane);
+    __threadfence();
+    __syncwarp();
+    const int f0 = work.block_of(first), parts = work.block_of(last) - f0 + 1;
+    int done = 0;
+    if (lane == 0) {
+      done = atomicAdd(&da.arrived[r], 1) == parts - 1;
+      if (done) {
+        da.arrived[r] = 0;
+        if (parts > 4) sm.finish[kind] = r;
+        __threadfence();
+      }
+    }
+    done = __shfl_sync(0xffffffffu, done, 0);
+    if (done && parts <= 4) {
+      st.clear();
+      for (int p = 0; p < parts; p += 2) {
+        const float* p0 = partial(f0, p, first);
+        st.fold_two(p0, p + 1 < parts ? partial(f0, p + 1, first) : p0, p + 1 < parts, lane);
+      }
+      write_run(r);
+    }
+  };
   // ---- runs that go on past this warp's slice (or came from another block):
   // the warp where the block's part of the run starts folds in the others'
-  const bool mine = ok && x0 < x1 && max(run_first, b0) >= x0 &&
-                    (run_last >= x1 || run_first < b0);
-  if (mine) {
+  if (ok && x0 < x1 && max(run_first, b0) >= x0 && (run_last >= x1 || run_first < b0)) {
     const int end = min(run_last + 1, b1);
-    for (int w = warp + 1; w < kDecWarps; ++w) {
-      const int w0 = b0 + static_cast<int>(static_cast<long long>(w) * span / kDecWarps);
-      const int w1 = b0 + static_cast<int>(static_cast<long long>(w + 1) * span / kDecWarps);
+    for (int w = warp + 1; w < W; ++w) {
+      const int w0 = b0 + w * span / W, w1 = b0 + (w + 1) * span / W;
       if (w0 < w1 && w0 < end) st.fold_from(sm.part[w], lane);
     }
-    const int i = run / heads, h = run - i * heads;
-    if (run_first >= b0 && run_last < b1) {
-      const int tok = a.start ? a.start[i] : i;
-      st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
-    } else {
-      publish(run, run_first, run_last, run_first >= b0 ? 1 : 0);
-    }
+    if (run_first >= b0 && run_last < b1) write_run(run);
+    else publish(run, run_first, run_last, run_first >= b0 ? 1 : 0);
+  }
+  if (sm.ended[0] >= 0 && warp == (sm.ended[3] + W / 2) % W) {
+    st.clear();
+    st.fold_from(sm.part[sm.ended[3]], lane);
+    publish(sm.ended[0], sm.ended[1], sm.ended[2], 0);
   }
   __syncthreads();
-  // ---- the last of a run's blocks merges its partials, all warps together
+  // ---- runs of many blocks: all warps merge their partials together
 #pragma unroll 1
   for (int f = 0; f < 2; ++f) {
     const int r = sm.finish[f];
@@ -697,21 +881,16 @@ __global__ void __launch_bounds__(kDecThreads, 1) kv8_decode_kernel(
     const int first = sm.prefix[i] + h * tiles, f0 = work.block_of(first);
     const int parts = work.block_of(first + tiles - 1) - f0 + 1;
     st.clear();
-    for (int p = warp; p < parts; p += kDecWarps) {
-      const int slot = 2 * (f0 + p) + (first >= work.begin(f0 + p) ? 1 : 0);
-      const float* src = da.part + static_cast<long long>(slot) * Sh::kPartFloats;
-      float o2[HD / 4];
-      const float m2 = __ldcg(src + lane), l2 = __ldcg(src + 32 + lane);
-#pragma unroll
-      for (int d = 0; d < HD / 4; ++d) o2[d] = __ldcg(src + (2 + d) * 32 + lane);
-      st.fold(m2, l2, o2);
+    for (int p = warp; p < parts; p += 2 * W) {
+      const bool two = p + W < parts;
+      const float* p0 = partial(f0, p, first);
+      st.fold_two(p0, two ? partial(f0, p + W, first) : p0, two, lane);
     }
     st.save(sm.part[warp], lane);
     __syncthreads();
     if (warp == 0) {
-      for (int w = 1; w < kDecWarps; ++w) st.fold_from(sm.part[w], lane);
-      const int tok = a.start ? a.start[i] : i;
-      st.write(static_cast<T*>(a.out) + tok * a.out_stride + h * G * HD, lane, G);
+      for (int w = 1; w < W; ++w) st.fold_from(sm.part[w], lane);
+      write_run(r);
     }
     __syncthreads();
   }

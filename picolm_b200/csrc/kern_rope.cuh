@@ -25,23 +25,29 @@ namespace pl {
 constexpr int kRopeThreads = 256;
 constexpr int kRopeRows = 8;  // rows per block, at most
 
-// cosine and sine of pair i at position pos, times the gain, rounded once
-// from FP64 to FP32
-__device__ __forceinline__ float2 rope_cs(const pl_rope& r, int i, int pos) {
+// Cosine and sine of a pair at position pos, times the gain, rounded once
+// from FP64 to FP32.
+__device__ __forceinline__ float2 rope_cs(double half_turns, double gain, int pos) {
   double s, c;
-  sincospi(r.half_turns[i] * static_cast<double>(pos), &s, &c);
-  return make_float2(static_cast<float>(c * r.gain), static_cast<float>(s * r.gain));
+  sincospi(half_turns * static_cast<double>(pos), &s, &c);
+  return make_float2(static_cast<float>(c * gain), static_cast<float>(s * gain));
+}
+__device__ __forceinline__ float2 rope_cs(const pl_rope& r, int i, int pos) {
+  return rope_cs(r.half_turns[i], r.gain, pos);
 }
 
 // The same in FP32 after an exact reduction to [-1, 1] half turns in FP64:
 // within 2e-7 of rope_cs, at a tenth of its time.  For q, which no rounding
 // to 8 bits follows.
-__device__ __forceinline__ float2 rope_cs_fast(const pl_rope& r, int i, int pos) {
-  const double x = r.half_turns[i] * static_cast<double>(pos);
+__device__ __forceinline__ float2 rope_cs_fast(double half_turns, double gain, int pos) {
+  const double x = half_turns * static_cast<double>(pos);
   float s, c;
   sincospif(static_cast<float>(x - 2.0 * rint(0.5 * x)), &s, &c);
-  const float g = static_cast<float>(r.gain);
+  const float g = static_cast<float>(gain);
   return make_float2(c * g, s * g);
+}
+__device__ __forceinline__ float2 rope_cs_fast(const pl_rope& r, int i, int pos) {
+  return rope_cs_fast(r.half_turns[i], r.gain, pos);
 }
 
 // Eight consecutive elements as FP32 (16-byte aligned FP16 / BF16, 32-byte

@@ -150,7 +150,7 @@ size_t plan_bytes(const pl_kv8* c) {  // src, dst, mark: one int a page each
 // One-token attention: two partials a block, then an arrival counter for each
 // entry and head.
 size_t part_bytes(const pl_kv8* c) {
-  return static_cast<size_t>(2) * kMaxBlocks * 32 * (c->head_dim / 4 + 2) * 4;
+  return static_cast<size_t>(2) * kMaxBlocks * (8 * c->head_dim + 16) * 4;
 }
 size_t arrive_bytes(const pl_kv8* c) {
   return static_cast<size_t>(pl::kPlanSeqs) * c->n_kv_heads * 4;
@@ -256,29 +256,63 @@ struct Read {
   }
 };
 
+// One token an entry; with k and v, they are appended by the same launch.
+template <typename T, int HD, int FMT, bool APPEND>
+int run_decode(const pl_kv8* c, pl::Kv8DecodeArgs d, void* st) {
+  d.part = work_part(c);
+  d.arrived = work_arrived(c);
+  CUtensorMap tm;
+  int rc = codes_map(c, pl::DecShape<HD>::kTileRows, &tm);
+  if (rc) return rc;
+  constexpr int smem = static_cast<int>(sizeof(pl::DecSmem<HD>)) + 1024;
+  static_assert(smem <= 227 * 1024, "shared memory of the one-token attention");
+  static std::atomic<unsigned long long> done{0};
+  auto kern = pl::kv8_decode_kernel<T, HD, FMT, APPEND>;
+  if ((rc = allow_smem(kern, smem, done))) return rc;
+  const int blocks = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
+  return launch(kern, dim3(blocks), pl::DecShape<HD>::kThreads, smem, st, true, d, tm);
+}
+
 template <typename T, int HD, int FMT>
 struct Attend {
   static int run(const pl_kv8* c, const pl::Kv8AttnArgs& a, void* st) {
     if (a.max_tok == 1) {
-      pl::Kv8DecodeArgs d;
+      pl::Kv8DecodeArgs d = {};
       d.a = a;
-      d.part = work_part(c);
-      d.arrived = work_arrived(c);
-      CUtensorMap tm;
-      int rc = codes_map(c, pl::DecShape<HD>::kTileRows, &tm);
-      if (rc) return rc;
-      constexpr int smem = static_cast<int>(sizeof(pl::DecSmem<HD>)) + 1024;
-      static_assert(smem <= 227 * 1024, "shared memory of the one-token attention");
-      static std::atomic<unsigned long long> done{0};
-      auto kern = pl::kv8_decode_kernel<T, HD, FMT>;
-      if ((rc = allow_smem(kern, smem, done))) return rc;
-      const int blocks = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
-      return launch(kern, dim3(blocks), pl::kDecThreads, smem, st, true, d, tm);
+      return run_decode<T, HD, FMT, false>(c, d, st);
     }
     return launch(pl::kv8_attend_plain_kernel<T, HD, FMT>, dim3(a.max_tok, c->n_kv_heads, a.n),
                   pl::kPlainThreads, 0, st, false, a);
   }
 };
+
+template <typename T, int HD, int FMT>
+struct Decode {
+  static int run(const pl_kv8* c, const pl::Kv8DecodeArgs& d, void* st) {
+    return run_decode<T, HD, FMT, true>(c, d, st);
+  }
+};
+
+pl::Kv8AttnArgs attn_args(const pl_kv8* c, int layer, int n, const int* d_seqs, const int* d_start,
+                          int total, int max_tok, const void* d_q, long long q_stride, void* d_out,
+                          long long out_stride) {
+  pl::Kv8AttnArgs a;
+  a.g = geo(c, layer);
+  a.rope = c->rope;
+  a.n = n;
+  a.total = total;
+  a.max_tok = max_tok;
+  a.n_heads = c->n_heads;
+  a.group = c->n_heads / c->n_kv_heads;
+  a.seqs = d_seqs;
+  a.start = d_start;
+  a.q = d_q;
+  a.out = d_out;
+  a.q_stride = q_stride;
+  a.out_stride = out_stride;
+  a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(double(c->head_dim)));
+  return a;
+}
 
 int plan(const pl_kv8* c, int op, int n, const int* a, const int* b, bool moves, void* stream) {
   pl::Kv8PlanArgs p;
@@ -521,37 +555,29 @@ int pl_kv8_attend_dev(const pl_kv8* c, int layer, int n, const int* d_seqs, cons
   if (!good_rows(d_q, q_stride, c->n_heads, c->head_dim, dtype) ||
       !good_rows(d_out, out_stride, c->n_heads, c->head_dim, dtype))
     return PL_EARG;
-  pl::Kv8AttnArgs a;
-  a.g = geo(c, layer);
-  a.rope = c->rope;
-  a.n = n;
-  a.total = total;
-  a.max_tok = max_tok;
-  a.n_heads = c->n_heads;
-  a.group = c->n_heads / c->n_kv_heads;
-  a.seqs = d_seqs;
-  a.start = d_start;
-  a.q = d_q;
-  a.out = d_out;
-  a.q_stride = q_stride;
-  a.out_stride = out_stride;
-  a.score_scale = static_cast<float>(1.4426950408889634 / std::sqrt(double(c->head_dim)));
-  return by_type<Attend>(c, dtype, a, stream);
+  return by_type<Attend>(c, dtype, attn_args(c, layer, n, d_seqs, d_start, total, max_tok, d_q,
+                                             q_stride, d_out, out_stride), stream);
 }
 
 int pl_kv8_decode_dev(const pl_kv8* c, int layer, int n, const int* d_seqs, int dtype,
                       const void* d_q, long long q_stride, const void* d_k, long long k_stride,
                       const void* d_v, long long v_stride, void* d_out, long long out_stride,
                       void* stream) {
-  const int one = n > 0 ? 1 : 0;
-  if (n > 0 && c && (!good_rows(d_q, q_stride, c->n_heads, c->head_dim, dtype) ||
-                     !good_rows(d_out, out_stride, c->n_heads, c->head_dim, dtype)))
-    return PL_EARG;  // before the append changes the cache
-  const int rc = pl_kv8_append_dev(c, layer, n, d_seqs, nullptr, n, 1, dtype, d_k, k_stride, d_v,
-                                   v_stride, stream);
-  if (rc || !one) return rc;
-  return pl_kv8_attend_dev(c, layer, n, d_seqs, nullptr, n, 1, dtype, d_q, q_stride, d_out,
-                           out_stride, stream);
+  bool none = false;
+  const int rc = check_call(c, layer, n, d_seqs, nullptr, n, 1, dtype, &none);
+  if (rc || none) return rc;
+  if (!good_rows(d_q, q_stride, c->n_heads, c->head_dim, dtype) ||
+      !good_rows(d_k, k_stride, c->n_kv_heads, c->head_dim, dtype) ||
+      !good_rows(d_v, v_stride, c->n_kv_heads, c->head_dim, dtype) ||
+      !good_rows(d_out, out_stride, c->n_heads, c->head_dim, dtype))
+    return PL_EARG;
+  pl::Kv8DecodeArgs d = {};
+  d.a = attn_args(c, layer, n, d_seqs, nullptr, n, 1, d_q, q_stride, d_out, out_stride);
+  d.k = d_k;
+  d.v = d_v;
+  d.k_stride = k_stride;
+  d.v_stride = v_stride;
+  return by_type<Decode>(c, dtype, d, stream);
 }
 
 int pl_kv8_read_dev(const pl_kv8* c, int layer, int n, const int* d_seqs, const int* d_row0,
