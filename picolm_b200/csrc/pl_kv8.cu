@@ -12,6 +12,7 @@
 #include "../../include/pl_attn.h"
 #include "kern_kv8.cuh"
 #include "kern_kv8_attn.cuh"
+#include "kern_kv8_chunk.cuh"
 #include "kern_rope.cuh"
 #include "pl_kv8.h"
 
@@ -67,7 +68,7 @@ int sm_count() {
   return n;
 }
 
-// Blocks of a one-token attention grid, at most (the workspace holds two
+// Blocks of an attention grid, at most (the workspace holds two
 // partials for each).
 constexpr int kMaxBlocks = 160;
 
@@ -147,14 +148,12 @@ size_t plan_bytes(const pl_kv8* c) {  // src, dst, mark: one int a page each
   return (static_cast<size_t>(c->n_pages) * 4 + 255) / 256 * 256 * 3;
 }
 
-// One-token attention: two partials a block, then an arrival counter for each
-// entry and head.
+// Attention: two partials a block (of two 128-row tiles, or of one token's
+// heads, which are smaller), then an arrival counter for each block.
 size_t part_bytes(const pl_kv8* c) {
-  return static_cast<size_t>(2) * kMaxBlocks * (8 * c->head_dim + 16) * 4;
+  return static_cast<size_t>(2) * kMaxBlocks * 2 * pl::kChRows * (c->head_dim + 2) * 4;
 }
-size_t arrive_bytes(const pl_kv8* c) {
-  return static_cast<size_t>(pl::kPlanSeqs) * c->n_kv_heads * 4;
-}
+size_t arrive_bytes(const pl_kv8*) { return static_cast<size_t>(kMaxBlocks) * 4; }
 
 size_t work_bytes(const pl_kv8* c) {
   return sizeof(pl::Kv8Head) + plan_bytes(c) + part_bytes(c) + arrive_bytes(c);
@@ -281,8 +280,19 @@ struct Attend {
       d.a = a;
       return run_decode<T, HD, FMT, false>(c, d, st);
     }
-    return launch(pl::kv8_attend_plain_kernel<T, HD, FMT>, dim3(a.max_tok, c->n_kv_heads, a.n),
-                  pl::kPlainThreads, 0, st, false, a);
+    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int smem = static_cast<int>(sizeof(pl::ChSmem<HD, PARTS>)) + 1024;
+    static_assert(smem <= 227 * 1024, "shared memory of the chunk attention");
+    static std::atomic<unsigned long long> done{0};
+    auto kern = pl::kv8_chunk_kernel<T, HD, FMT>;
+    pl::Kv8ChunkArgs ch = {};
+    ch.a = a;
+    ch.part = work_part(c);
+    ch.arrived = work_arrived(c);
+    int rc = allow_smem(kern, smem, done);
+    if (rc) return rc;
+    const int blocks = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
+    return launch(kern, dim3(blocks), pl::kChThreads, smem, st, true, ch);
   }
 };
 

@@ -220,6 +220,16 @@ def test_nan_stays_where_it_is():
     want[80:100, 2:] = True
     want[150, 0] = True
     assert torch.equal(bad, want)
+    # the same for V, and one token at a time
+    c.scales[int(c.table[0, 1]), 0, 1, 0, 1] = 0.02
+    c.scales[int(c.table[0, 1]), 0, 0, 1, 1] = math.nan   # rows 80..95, head 0, V
+    q[150, 0] = 1.0
+    out = c.attend([0, 1], [100, 100], q, torch.empty_like(q), pb.PL_F32).view(200, 4, 64)
+    want[:] = False
+    want[80:100, :2] = True
+    assert torch.equal(torch.isnan(out).any(-1), want)
+    out = c.attend([0, 1], [1, 1], q[:2], torch.empty_like(q[:2]), pb.PL_F32).view(2, 4, 64)
+    assert torch.isnan(out).any(-1).tolist() == [[True, True, False, False], [False] * 4]
 
 
 @pytest.mark.parametrize("seqs,length", [(1, 20000), (3, 9001)])
