@@ -153,19 +153,23 @@ size_t plan_bytes(const pl_kv8* c) {  // src, dst, mark: one int a page each
 size_t part_bytes(const pl_kv8* c) {
   return static_cast<size_t>(2) * kMaxBlocks * 2 * pl::kChRows * (c->head_dim + 2) * 4;
 }
+// FP32 sums of the chunk attention's output tiles, one pair of tiles a block.
+size_t sum_bytes(const pl_kv8* c) {
+  return static_cast<size_t>(kMaxBlocks) * 2 * pl::kChRows * c->head_dim * 4;
+}
 size_t arrive_bytes(const pl_kv8*) { return static_cast<size_t>(kMaxBlocks) * 4; }
 
 size_t work_bytes(const pl_kv8* c) {
-  return sizeof(pl::Kv8Head) + plan_bytes(c) + part_bytes(c) + arrive_bytes(c);
+  return sizeof(pl::Kv8Head) + plan_bytes(c) + part_bytes(c) + sum_bytes(c) + arrive_bytes(c);
 }
 
 float* work_part(const pl_kv8* c) {
   return reinterpret_cast<float*>(static_cast<uint8_t*>(c->work) + sizeof(pl::Kv8Head) +
                                   plan_bytes(c));
 }
+float* work_sums(const pl_kv8* c) { return work_part(c) + part_bytes(c) / 4; }
 int* work_arrived(const pl_kv8* c) {
-  return reinterpret_cast<int*>(static_cast<uint8_t*>(c->work) + sizeof(pl::Kv8Head) +
-                                plan_bytes(c) + part_bytes(c));
+  return reinterpret_cast<int*>(work_sums(c) + sum_bytes(c) / 4);
 }
 
 // Every call on a cache: its shape, its memory and the current device.
@@ -288,6 +292,7 @@ struct Attend {
     pl::Kv8ChunkArgs ch = {};
     ch.a = a;
     ch.part = work_part(c);
+    ch.sums = work_sums(c);
     ch.arrived = work_arrived(c);
     int rc = allow_smem(kern, smem, done);
     if (rc) return rc;

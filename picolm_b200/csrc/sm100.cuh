@@ -85,6 +85,18 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
+// The same in a few instructions: for kernels with many waits in their
+// loops, where the unrolled polling above (6 KB of code a wait) pushes the
+// loop itself out of the instruction cache.
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer(), lim = wait_limit_ns();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity))
+    if (globaltimer() - t0 > lim) return false;
+  return true;
+}
+
 // ---------------------------------------------------------------- fences
 __device__ __forceinline__ void fence_proxy_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
