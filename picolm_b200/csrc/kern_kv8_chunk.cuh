@@ -122,6 +122,7 @@ struct ChSmem {
   uint8_t raw[Sh::kRaw][Sh::kRawBytes];
   float raw_scale[Sh::kRaw][2][kBlocksPerPage];  // of K and V, beside K's codes
   float scale[8][2][Sh::kBlocks];  // of tile n in n % 8, K and V
+  uint32_t bad[8];                 // blocks of it with a scale that is not finite
   float2 base[8][HD / 2];          // a softmax warp's cosines of its slot's first position
   float2 step[24][HD / 2];         // of 0..7 and of 0, 8, .. 120 tokens further
   float q_scale[2][kChRows];
@@ -177,15 +178,6 @@ __device__ __forceinline__ Raw8<T> raw8(const T* p) {
 template <typename T>
 __device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&x)[8]) {
   load8(reinterpret_cast<const T*>(r.v), x);
-}
-
-// What a score of a block is multiplied by: its K scale times the row's.  A
-// masked -inf times 0 would be NaN, and so would a NaN scale make it: both
-// become a tiny factor (the codes under a 0 scale are 0; the rows that see a
-// NaN block are made NaN apart).
-__device__ __forceinline__ float score_unit(float scale, float q_scale) {
-  const float f = scale * q_scale;
-  return f > 0.f && f < INFINITY ? f : 1e-30f;
 }
 
 template <typename T, int HD, int FMT>
@@ -535,15 +527,12 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         for (int c = 0; c < kChunks; ++c) in[c] = src[c * 128];
 #pragma unroll
         for (int c = 0; c < kChunks; ++c) {
-          const int row = row0 + c * kRowStep;
-          // (rows past the end: anything may be there, NaN codes too)
-          if (left < BN && row >= left) in[c] = make_uint4(0, 0, 0, 0);
           const uint32_t w4[4] = {in[c].x, in[c].y, in[c].z, in[c].w};
           uint32_t o[8];
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            o[2 * q] = codes_bits2<FMT, 0x10>(w4[q]);
-            o[2 * q + 1] = codes_bits2<FMT, 0x32>(w4[q]);
+            o[2 * q] = codes_half2<FMT, 0x10>(w4[q]);
+            o[2 * q + 1] = codes_half2<FMT, 0x32>(w4[q]);
           }
           // elements 16 ch ..: chunks 2ch, 2ch + 1 of a 64-element half; rows
           // are kRowStep (a multiple of 8) apart, so the swizzle is row0's
@@ -552,10 +541,23 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           *reinterpret_cast<uint4*>(dst + c * kRowStep * 128 + (at0 ^ 16)) =
               make_uint4(o[4], o[5], o[6], o[7]);
         }
-        if (!is_v && pt < 2 * Sh::kBlocks) {
-          const int kv = pt / Sh::kBlocks, b = pt % Sh::kBlocks;
-          sm.scale[n & 7][kv][b] =
-              b * kBlock < left ? sm.raw_scale[rs][kv][b] * code_unit<FMT>() : 0.f;
+        if (left < BN) {  // rows past the end: anything was there, NaN codes too
+#pragma unroll 1
+          for (int row = row0, o = 0; row < BN; row += kRowStep, o += kRowStep * 128)
+            if (row >= left) {
+              *reinterpret_cast<uint4*>(dst + o + at0) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(dst + o + (at0 ^ 16)) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        if (!is_v && pt < 32) {
+          // A scale that is not finite becomes 0 and leaves a bit: rows that see
+          // its block are made NaN, and 0 times what a mask hides stays 0.
+          const int kv = pt / Sh::kBlocks & 1, b = pt % Sh::kBlocks;
+          const float f = b * kBlock < left ? sm.raw_scale[rs][kv][b] : 0.f;
+          const uint32_t odd =
+              __ballot_sync(0xffffffffu, pt < 2 * Sh::kBlocks && !(f < INFINITY));
+          if (pt < 2 * Sh::kBlocks) sm.scale[n & 7][kv][b] = f < INFINITY ? f : 0.f;
+          if (pt == 0) sm.bad[n & 7] = (odd | odd >> Sh::kBlocks) & ((1u << Sh::kBlocks) - 1);
         }
         fence_proxy_async_smem();
         __syncwarp();
@@ -590,6 +592,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       const int p_min = g.len - g.n_tok + tok_x;   // position of the slot's first token
       const int pos = real ? p_min + row_tok : -1;
       float m_used = -INFINITY, l_run = 0.f, ref = kMinRef, q_scale = 0.f;
+      float unit = kChBase / kMinRef;  // what V's scales are multiplied by
       float m_sum = -INFINITY, ref_sum = kMinRef;  // of the sums outside TMEM
       const long long out_row = static_cast<long long>(g.tok0) + tok_x + row_tok;
       const int head_el = (g.h * G + row_head) * HD;
@@ -759,6 +762,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           sk[0] = fk.x, sk[1] = fk.y, sk[2] = fk.z, sk[3] = fk.w;
           sv[0] = fv.x, sv[1] = fv.y, sv[2] = fv.z, sv[3] = fv.w;
         }
+        // what a block's scores are multiplied by; never 0, which would make a
+        // masked -inf NaN (the codes under a scale of 0 are 0)
+#pragma unroll
+        for (int b = 0; b < Sh::kBlocks; ++b) sk[b] = fmaxf(sk[b] * q_scale, 1e-30f);
+        if (const uint32_t bad = sm.bad[n & 7]) {
+          if (lim >= 16 * (__ffs(bad) - 1)) l_run = NAN;
+        }
         if (need_mask) {
 #pragma unroll
           for (int c = 0; c < BN; ++c) {
@@ -776,16 +786,9 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
                                     max3(at(6), at(7), at(8))),
                                max3(at(9), at(10), at(11)),
                                max3(max3(at(12), at(13), at(14)), at(15), at(15)));
-          m_tile = fmaxf(m_tile, z * score_unit(sk[b], q_scale));
+          m_tile = fmaxf(m_tile, z * sk[b]);
         }
-        // a NaN scale makes the rows that see its block NaN, and no others
-        float top_v = 0.f;
-#pragma unroll
-        for (int b = 0; b < Sh::kBlocks; ++b) {
-          const bool bad_v = !(sv[b] < INFINITY);
-          if ((bad_v || !(sk[b] < INFINITY)) && lim >= 16 * b) l_run = NAN;
-          top_v = fmaxf(top_v, bad_v ? 0.f : sv[b]);
-        }
+        const float top_v = max3(fmaxf(sv[0], sv[1]), sv[2], sv[3]);
         const bool rescale = __any_sync(0xffffffffu, m_tile > m_used + kChRescaleLog2) ||
                              top_v > kChRefGrowth * ref;
         const bool moved = PARTS == 2 && j > 0 && j % Sh::kFlushTiles == 0;
@@ -802,6 +805,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           l_run *= alpha;
           m_used = m_new;
           ref = ref_new;
+          unit = kChBase / ref;
           if (j > 0 && !moved) {
 #pragma unroll
             for (int d0 = 0; d0 < HD; d0 += 16) {
@@ -817,7 +821,6 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
             }
           }
         }
-        const float unit = kChBase / ref;
         const float m_safe = m_used == -INFINITY ? 0.f : m_used;
         const float2 nm2 = make_float2(-m_safe, -m_safe);
         float2 rs2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -827,8 +830,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           uint32_t hi[16], lo[16];
 #pragma unroll
           for (int b = 2 * q; b < 2 * q + 2; ++b) {
-            const float kb = score_unit(sk[b], q_scale);
-            const float vb = sv[b] < INFINITY ? sv[b] * unit : 0.f;
+            const float kb = sk[b], vb = sv[b] * unit;
 #pragma unroll
             for (int e = 8 * b; e < 8 * b + 8; ++e) {
               const float2 arg =

@@ -85,14 +85,25 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   }
 }
 
-// The same in a few instructions: for kernels with many waits in their
-// loops, where the unrolled polling above (6 KB of code a wait) pushes the
-// loop itself out of the instruction cache.
+// The same in a few instructions, and asleep for up to 20 us at a time: for
+// kernels with many waiting warps beside working ones.  (The unrolled polling
+// above is 6 KB of code a wait, and takes issue slots while it waits.)
+__device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity), "r"(20000)
+      : "memory");
+  return ok != 0;
+}
 __device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity) {
-  if (mbar_try_wait(bar, parity)) return true;
+  if (mbar_sleep_wait(bar, parity)) return true;
   const uint64_t t0 = globaltimer(), lim = wait_limit_ns();
 #pragma unroll 1
-  while (!mbar_try_wait(bar, parity))
+  while (!mbar_sleep_wait(bar, parity))
     if (globaltimer() - t0 > lim) return false;
   return true;
 }
