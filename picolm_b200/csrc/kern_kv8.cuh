@@ -137,37 +137,62 @@ __device__ __forceinline__ bool kv8_entry(const Kv8Geo& g, int i, int total, int
 
 constexpr int kAppendThreads = 256;
 
-// Elements [e, e + 8) of one head row, rotated when `cs` is set (K).
-template <typename T, int HD>
-__device__ __forceinline__ void load_rotated(const T* x, int e, const pl_rope& r, const float2* cs,
-                                             float (&y)[8]) {
+// Elements [e, e + 8) of a head row as they are, and the run that rotates
+// with them (Qwen).
+template <typename T>
+__device__ __forceinline__ void load_pair8(const T* x, int e, const pl_rope& r, bool rotated,
+                                           float (&y)[8], float (&z)[8]) {
   load8(x + e, y);
-  if (!cs || e >= r.dim) return;
+  if (!rotated || r.type == PL_ROPE_LLAMA || e >= r.dim) return;
   const int half = r.dim >> 1;
-  if (r.type == PL_ROPE_LLAMA) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (e + 2 * j >= r.dim) break;
-      const float2 c = cs[(e >> 1) + j];
-      const float a = y[2 * j], b = y[2 * j + 1];
-      y[2 * j] = __fsub_rn(__fmul_rn(a, c.x), __fmul_rn(b, c.y));
-      y[2 * j + 1] = __fadd_rn(__fmul_rn(a, c.y), __fmul_rn(b, c.x));
-    }
+  if (half % 8 == 0) {
+    load8(x + (e < half ? e + half : e - half), z);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int d = e + j;
-      if (d >= r.dim) break;
-      if (d < half) {
-        const float2 c = cs[d];
-        y[j] = __fsub_rn(__fmul_rn(y[j], c.x), __fmul_rn(to_f32(x[d + half]), c.y));
-      } else {
-        const float2 c = cs[d - half];
-        y[j] = __fadd_rn(__fmul_rn(to_f32(x[d - half]), c.y), __fmul_rn(y[j], c.x));
-      }
+      z[j] = d < r.dim ? to_f32(x[d < half ? d + half : d - half]) : 0.f;
     }
   }
 }
+// y rotated by cs[pair], with the roundings of rope().
+__device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const float2* cs,
+                                             float (&y)[8], const float (&z)[8]) {
+  if (e >= r.dim) return;
+  const int half = r.dim >> 1;
+  if (r.type == PL_ROPE_LLAMA) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (e + 2 * j < r.dim) rope_one(y[2 * j], y[2 * j + 1], cs[(e >> 1) + j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int d = e + j;
+      if (d < half)
+        y[j] = __fsub_rn(__fmul_rn(y[j], cs[d].x), __fmul_rn(z[j], cs[d].y));
+      else if (d < r.dim)
+        y[j] = __fadd_rn(__fmul_rn(z[j], cs[d - half].y), __fmul_rn(y[j], cs[d - half].x));
+    }
+  }
+}
+
+// x / by, correctly rounded, from the reciprocal (Markstein, 1990: with inv
+// the rounded reciprocal of by, one correction by the exact remainder gives
+// the rounded quotient), where nothing comes near the ends of the range.
+struct Quotient {
+  float by, inv;
+  bool plain;
+  __device__ __forceinline__ explicit Quotient(float d) {
+    by = d;
+    inv = __fdiv_rn(1.f, d);
+    plain = !(d > 1e-25f && d < 1e25f);
+  }
+  __device__ __forceinline__ float operator()(float x) const {
+    if (plain) return __fdiv_rn(x, by);
+    const float q = __fmul_rn(x, inv);
+    return fmaf(fmaf(-q, by, x), inv, q);
+  }
+};
 
 // Block (x, y) of the grid: the x-th block of 16 rows that entry y touches,
 // all heads, K and V.  A warp takes one (head, K or V): its 16 rows live in
@@ -177,11 +202,19 @@ __device__ __forceinline__ void load_rotated(const T* x, int e, const pl_rope& r
 // rows raise the scale (code' = round(code * old / new)).  A row with a
 // NaN or infinity makes the scale NaN: the whole block then reads as NaN
 // rather than as finite numbers that were never written.
+//
+// Cosines are FP64 and rounded once, so that codes do not depend on how a
+// row was appended; a block of rows takes two sincospi a pair (its first
+// row's and one row's step) and turns from row to row by FP64 products.
 template <typename T, int HD, int FMT>
-__global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(
+__global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
     const __grid_constant__ Kv8AppendArgs a) {
   __shared__ float2 s_cs[kBlock][HD / 2];
+  __shared__ double s_turns[HD / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x < HD / 2) s_turns[threadIdx.x] = a.rope.half_turns[threadIdx.x];
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Kv8Entry e;
   if (!kv8_entry(a.g, blockIdx.y, a.total, a.max_tok, a.seqs, a.start, e) || e.len < e.n_tok) {
     if (threadIdx.x == 0 && blockIdx.x == 0) atomicOr(&a.g.head->err, ERR_BAD_ARG);
@@ -197,9 +230,25 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(
   }
   const int lo = max(row0 - blk * kBlock, 0), hi = min(e.len - blk * kBlock, kBlock);  // new rows
   const int pairs = a.rope.dim >> 1;
-  for (int t = threadIdx.x; t < (hi - lo) * pairs; t += kAppendThreads) {
-    const int r = t / pairs, i = t - r * pairs;
-    s_cs[lo + r][i] = rope_cs(a.rope, i, blk * kBlock + lo + r);
+  __syncthreads();
+  {
+    // thread (pair, group): rows lo + group * per .. of the pair
+    constexpr int kGroups = kAppendThreads / (HD / 2);
+    const int i = threadIdx.x % (HD / 2), group = threadIdx.x / (HD / 2);
+    const int per = (hi - lo + kGroups - 1) / kGroups, r0 = lo + group * per;
+    const int r1 = min(r0 + per, hi);
+    if (i < pairs && r0 < r1) {
+      double s, c, ss = 0.0, sc = 1.0;
+      sincospi(s_turns[i] * static_cast<double>(blk * kBlock + r0), &s, &c);
+      if (r1 - r0 > 1) sincospi(s_turns[i], &ss, &sc);
+      for (int r = r0; r < r1; ++r) {
+        s_cs[r][i] = make_float2(static_cast<float>(c * a.rope.gain),
+                                 static_cast<float>(s * a.rope.gain));
+        const double nc = c * sc - s * ss;
+        s = s * sc + c * ss;
+        c = nc;
+      }
+    }
   }
   __syncthreads();
   constexpr int kLanesPerRow = HD / 8, kRowsPerPass = 32 / kLanesPerRow;
@@ -217,21 +266,30 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(
     float x[kPasses][8];
     uint32_t top = 0;  // bits of the largest absolute value: NaN sorts above infinity
 #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int r = p * kRowsPerPass + lane / kLanesPerRow;
-      if (r >= lo && r < hi) {
-        const long long tok = e.tok0 + (blk * kBlock + r - row0);
-        load_rotated<T, HD>(src + tok * stride + h * HD, el, a.rope, kv ? nullptr : s_cs[r], x[p]);
+    for (int p0 = 0; p0 < kPasses; p0 += 2) {
+      float z[2][8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(fabsf(x[p][j])));
+      for (int p = p0; p < p0 + 2; ++p) {
+        const int r = p * kRowsPerPass + lane / kLanesPerRow;
+        if (r >= lo && r < hi)
+          load_pair8(src + static_cast<long long>(e.tok0 + (blk * kBlock + r - row0)) * stride +
+                         h * HD, el, a.rope, kv == 0, x[p], z[p - p0]);
+      }
+#pragma unroll
+      for (int p = p0; p < p0 + 2; ++p) {
+        const int r = p * kRowsPerPass + lane / kLanesPerRow;
+        if (r >= lo && r < hi) {
+          if (kv == 0) rotate_pair8(el, a.rope, s_cs[r], x[p], z[p - p0]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(fabsf(x[p][j])));
+        }
       }
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    top = __reduce_max_sync(0xffffffffu, top);
     float s = __fdiv_rn(__uint_as_float(top), code_top<FMT>());
     if (top >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
     s = __uint_as_float(max(__float_as_uint(s), old_bits));
-    const float by = s > 0.f ? s : 1.f;
+    const Quotient over(s > 0.f ? s : 1.f);
     const bool grown = lo > 0 && __float_as_uint(s) != old_bits;
     const float ratio = s > 0.f ? __fdiv_rn(__uint_as_float(old_bits), s) : 1.f;
     __syncwarp();  // every lane has read the old scale
@@ -242,7 +300,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv8_append_kernel(
       uint2* at = reinterpret_cast<uint2*>(dst + r * HD);
       if (r >= lo && r < hi) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[p][j] = __fdiv_rn(x[p][j], by);
+        for (int j = 0; j < 8; ++j) x[p][j] = over(x[p][j]);
         *at = encode8<FMT>(x[p]);
       } else if (r < lo && grown) {
         float y[8];

@@ -108,41 +108,49 @@ __device__ __forceinline__ void from_f32(__nv_bfloat16* p, float x) { *p = __flo
 struct RopeRowsArgs {
   pl_rope rope;
   const int* pos;
-  int n, n_heads, n_kv_heads, adjoint, rows_per_block, vec;
+  int n, n_heads, n_kv_heads, adjoint, rows_per_block;
+  int units, per_head;   // vector units of a row, of a head
+  uint64_t per_head_inv; // ceil(2^32 / per_head)
   const void *q, *k;
   void *qo, *ko;
   long long q_stride, qo_stride, k_stride, ko_stride;  // elements between rows
 };
 
-// One head row of head_dim elements by pairs: the form of any dim, stride
-// and alignment.
-template <typename T>
-__device__ __forceinline__ void rope_pair_any(const RopeRowsArgs& a, const T* x, T* y, int i,
-                                              float2 cs) {
+// Cosines and sines of the block's rows, once for all heads.
+__device__ __forceinline__ void rope_rows_table(const RopeRowsArgs& a, int row0, int rows,
+                                                float2 (*s_cs)[PL_ROPE_MAX_PAIRS],
+                                                double* s_turns) {
   const int half = a.rope.dim >> 1;
-  const int ea = a.rope.type == PL_ROPE_LLAMA ? 2 * i : i;
-  const int eb = a.rope.type == PL_ROPE_LLAMA ? 2 * i + 1 : i + half;
-  const float xa = to_f32(x[ea]), xb = to_f32(x[eb]);
-  from_f32(y + ea, __fsub_rn(__fmul_rn(xa, cs.x), __fmul_rn(xb, cs.y)));
-  from_f32(y + eb, __fadd_rn(__fmul_rn(xa, cs.y), __fmul_rn(xb, cs.x)));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
-    const __grid_constant__ RopeRowsArgs a) {
-  __shared__ float2 s_cs[kRopeRows][PL_ROPE_MAX_PAIRS];
-  const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
-  const int row0 = blockIdx.x * a.rows_per_block;
-  const int rows = min(a.rows_per_block, a.n - row0);
+  for (int i = threadIdx.x; i < half; i += kRopeThreads) s_turns[i] = a.rope.half_turns[i];
+  __syncthreads();
   for (int t = threadIdx.x; t < rows * half; t += kRopeThreads) {
     const int r = t / half, i = t - r * half;
-    float2 cs = rope_cs(a.rope, i, a.pos[row0 + r]);
+    float2 cs = rope_cs(s_turns[i], a.rope.gain, a.pos[row0 + r]);
     if (a.adjoint) cs.y = -cs.y;
     s_cs[r][i] = cs;
   }
   __syncthreads();
+}
+
+// y = x rotated by cs, with the roundings of rope() (two products, a sum)
+__device__ __forceinline__ void rope_one(float& a, float& b, float2 cs) {
+  const float u = a, v = b;
+  a = __fsub_rn(__fmul_rn(u, cs.x), __fmul_rn(v, cs.y));
+  b = __fadd_rn(__fmul_rn(u, cs.y), __fmul_rn(v, cs.x));
+}
+
+// Any dim, stride and alignment: a unit is one pair, or one element past
+// dim, of one head.
+template <typename T>
+__global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
+    const __grid_constant__ RopeRowsArgs a) {
+  __shared__ float2 s_cs[kRopeRows][PL_ROPE_MAX_PAIRS];
+  __shared__ double s_turns[PL_ROPE_MAX_PAIRS];
+  const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int rows = min(a.rows_per_block, a.n - row0);
+  rope_rows_table(a, row0, rows, s_cs, s_turns);
   const int heads = a.n_heads + a.n_kv_heads;
-  // a unit is one pair, or one element past dim, of one head
   const int per_head = half + (hd - a.rope.dim);
   for (int t = threadIdx.x; t < rows * heads * per_head; t += kRopeThreads) {
     const int u = t % per_head, rh = t / per_head, h = rh % heads, r = rh / heads;
@@ -152,11 +160,85 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
                       : static_cast<const T*>(a.k) + row * a.k_stride + (h - a.n_heads) * hd;
     T* y = is_q ? static_cast<T*>(a.qo) + row * a.qo_stride + h * hd
                 : static_cast<T*>(a.ko) + row * a.ko_stride + (h - a.n_heads) * hd;
-    if (u < half)
-      rope_pair_any<T>(a, x, y, u, s_cs[r][u]);
-    else
+    if (u < half) {
+      const bool llama = a.rope.type == PL_ROPE_LLAMA;
+      const int ea = llama ? 2 * u : u, eb = llama ? 2 * u + 1 : u + half;
+      float xa = to_f32(x[ea]), xb = to_f32(x[eb]);
+      rope_one(xa, xb, s_cs[r][u]);
+      from_f32(y + ea, xa);
+      from_f32(y + eb, xb);
+    } else {
       y[a.rope.dim + u - half] = x[a.rope.dim + u - half];
+    }
   }
+}
+
+// Aligned rows.  A unit is eight elements of a head (LLaMA; past dim: copied)
+// or the two runs of eight that rotate together (Qwen, dim / 2 a multiple of
+// eight); a thread has the loads of four units under way.
+template <typename T, bool LLAMA>
+__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
+    const __grid_constant__ RopeRowsArgs a) {
+  __shared__ float2 s_cs[kRopeRows][PL_ROPE_MAX_PAIRS];
+  __shared__ double s_turns[PL_ROPE_MAX_PAIRS];
+  const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
+  const int row0 = blockIdx.x * a.rows_per_block;
+  const int rows = min(a.rows_per_block, a.n - row0);
+  const int all = a.units;
+  constexpr int U = 4;
+  const T* src[U];
+  T* dst[U];
+  int el[U], step = LLAMA ? 0 : half;  // from the first to the second run
+  float x[U][8], z[U][8];
+  // unit u of row r: its addresses; false past the row
+  auto find = [&](int u, int r, int k) {
+    const int h = static_cast<int>((static_cast<uint64_t>(u) * a.per_head_inv) >> 32);
+    const int c = u - h * a.per_head;
+    // Qwen: the runs below half, then those past dim
+    el[k] = LLAMA || c * 8 < half ? c * 8 : c * 8 + half;
+    const bool is_q = h < a.n_heads;
+    const long long row = row0 + r;
+    const long long at = static_cast<long long>(is_q ? h : h - a.n_heads) * hd + el[k];
+    src[k] = is_q ? static_cast<const T*>(a.q) + row * a.q_stride + at
+                  : static_cast<const T*>(a.k) + row * a.k_stride + at;
+    dst[k] = is_q ? static_cast<T*>(a.qo) + row * a.qo_stride + at
+                  : static_cast<T*>(a.ko) + row * a.ko_stride + at;
+  };
+  auto rotate = [&](int r, int k) {
+    const float2* cs = s_cs[r];
+    if constexpr (LLAMA) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (el[k] + 2 * i < a.rope.dim)
+          rope_one(x[k][2 * i], x[k][2 * i + 1], cs[(el[k] >> 1) + i]);
+    } else if (el[k] < half) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) rope_one(x[k][i], z[k][i], cs[el[k] + i]);
+      store8(dst[k] + step, z[k]);
+    }
+    store8(dst[k], x[k]);
+  };
+  // the first units are on their way while the cosines are computed
+  bool first = true;
+  for (int r = 0; r < rows; ++r)
+    for (int u0 = threadIdx.x; u0 < all || first; u0 += U * kRopeThreads) {
+#pragma unroll
+      for (int k = 0; k < U; ++k) {
+        const int u = u0 + k * kRopeThreads;
+        if (u < all) {
+          find(u, r, k);
+          load8(src[k], x[k]);
+          if (!LLAMA && el[k] < half) load8(src[k] + step, z[k]);
+        }
+      }
+      if (first) {
+        rope_rows_table(a, row0, rows, s_cs, s_turns);
+        first = false;
+      }
+#pragma unroll
+      for (int k = 0; k < U; ++k)
+        if (u0 + k * kRopeThreads < all) rotate(r, k);
+    }
 }
 
 }  // namespace pl

@@ -246,7 +246,7 @@ struct Append {
   static int run(const pl_kv8*, const pl::Kv8AppendArgs& a, void* st) {
     const int blocks = (a.max_tok + PL_KV8_BLOCK - 2) / PL_KV8_BLOCK + 1;
     return launch(pl::kv8_append_kernel<T, HD, FMT>, dim3(blocks, a.n), pl::kAppendThreads, 0, st,
-                  false, a);
+                  true, a);
   }
 };
 
@@ -434,16 +434,34 @@ int pl_rope_rows_dev(const pl_rope* r, int dtype, int n, const int* d_pos, int n
   a.qo_stride = q_out_stride;
   a.k_stride = k_stride;
   a.ko_stride = k_out_stride;
-  a.vec = 0;
   // as many rows a block as leave every SM a few blocks
-  int rows = n / (4 * sms);
+  const int rows = n / (4 * sms);
   a.rows_per_block = rows < 1 ? 1 : rows > pl::kRopeRows ? pl::kRopeRows : rows;
   const dim3 grid((n + a.rows_per_block - 1) / a.rows_per_block);
+  const int half = r->dim / 2;
+  const bool llama = r->type == PL_ROPE_LLAMA;
+  auto vec = [&](int heads, const void* p, long long s, const void* o, long long os) {
+    const long long e = static_cast<long long>(es);
+    return !heads || (aligned(p, 16) && aligned(o, 16) && s * e % 16 == 0 && os * e % 16 == 0);
+  };
+  const bool fast = (llama || half % 8 == 0) &&
+                    vec(n_heads, d_q, q_stride, d_q_out, q_out_stride) &&
+                    vec(n_kv_heads, d_k, k_stride, d_k_out, k_out_stride);
+  a.per_head = llama ? r->head_dim / 8 : half / 8 + (r->head_dim - r->dim) / 8;
+  a.units = a.per_head * (n_heads + n_kv_heads);
+  a.per_head_inv = fast ? ((1ull << 32) + a.per_head - 1) / a.per_head : 0;
+  auto go = [&](auto any, auto by_pairs, auto by_halves) {
+    return launch(!fast ? any : llama ? by_pairs : by_halves, grid, pl::kRopeThreads, 0, stream,
+                  false, a);
+  };
   if (dtype == PL_F32)
-    return launch(pl::rope_rows_kernel<float>, grid, pl::kRopeThreads, 0, stream, false, a);
+    return go(pl::rope_rows_any_kernel<float>, pl::rope_rows_kernel<float, true>,
+              pl::rope_rows_kernel<float, false>);
   if (dtype == PL_F16)
-    return launch(pl::rope_rows_kernel<__half>, grid, pl::kRopeThreads, 0, stream, false, a);
-  return launch(pl::rope_rows_kernel<__nv_bfloat16>, grid, pl::kRopeThreads, 0, stream, false, a);
+    return go(pl::rope_rows_any_kernel<__half>, pl::rope_rows_kernel<__half, true>,
+              pl::rope_rows_kernel<__half, false>);
+  return go(pl::rope_rows_any_kernel<__nv_bfloat16>, pl::rope_rows_kernel<__nv_bfloat16, true>,
+            pl::rope_rows_kernel<__nv_bfloat16, false>);
 }
 
 // ------------------------------------------------------------------- cache
