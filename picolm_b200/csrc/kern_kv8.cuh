@@ -141,17 +141,18 @@ constexpr int kAppendThreads = 256;
 // with them (Qwen).
 template <typename T>
 __device__ __forceinline__ void load_pair8(const T* x, int e, const pl_rope& r, bool rotated,
-                                           float (&y)[8], float (&z)[8]) {
-  load8(x + e, y);
+                                           Raw8<T>& y, Raw8<T>& z) {
+  y = raw8(x + e);
   if (!rotated || r.type == PL_ROPE_LLAMA || e >= r.dim) return;
   const int half = r.dim >> 1;
   if (half % 8 == 0) {
-    load8(x + (e < half ? e + half : e - half), z);
+    z = raw8(x + (e < half ? e + half : e - half));
   } else {
+    T* p = reinterpret_cast<T*>(&z);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int d = e + j;
-      z[j] = d < r.dim ? to_f32(x[d < half ? d + half : d - half]) : 0.f;
+      p[j] = x[d < half ? d + half : d < r.dim ? d - half : d];
     }
   }
 }
@@ -176,23 +177,13 @@ __device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const floa
   }
 }
 
-// x / by, correctly rounded, from the reciprocal (Markstein, 1990: with inv
-// the rounded reciprocal of by, one correction by the exact remainder gives
-// the rounded quotient), where nothing comes near the ends of the range.
-struct Quotient {
-  float by, inv;
-  bool plain;
-  __device__ __forceinline__ explicit Quotient(float d) {
-    by = d;
-    inv = __fdiv_rn(1.f, d);
-    plain = !(d > 1e-25f && d < 1e25f);
-  }
-  __device__ __forceinline__ float operator()(float x) const {
-    if (plain) return __fdiv_rn(x, by);
-    const float q = __fmul_rn(x, inv);
-    return fmaf(fmaf(-q, by, x), inv, q);
-  }
-};
+// x / by, correctly rounded, from the rounded reciprocal inv of by
+// (Markstein, 1990: one correction by the exact remainder gives the rounded
+// quotient), where nothing comes near the ends of the range.
+__device__ __forceinline__ float quotient(float x, float by, float inv) {
+  const float q = __fmul_rn(x, inv);
+  return fmaf(fmaf(-q, by, x), inv, q);
+}
 
 // Block (x, y) of the grid: the x-th block of 16 rows that entry y touches,
 // all heads, K and V.  A warp takes one (head, K or V): its 16 rows live in
@@ -264,45 +255,76 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
     const long long stride = kv ? a.v_stride : a.k_stride;
     const uint32_t old_bits = lo > 0 ? __float_as_uint(*sc) : 0u;
     float x[kPasses][8];
-    uint32_t top = 0;  // bits of the largest absolute value: NaN sorts above infinity
+    float top = 0.f;
+    uint32_t odd = 0;  // a NaN or infinity
+    const T* row_src = src + static_cast<long long>(e.tok0 + (blk * kBlock - row0) +
+                                                    lane / kLanesPerRow) * stride + h * HD;
+    const int r_lane = lane / kLanesPerRow;
+    constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // rows under way
 #pragma unroll
-    for (int p0 = 0; p0 < kPasses; p0 += 2) {
-      float z[2][8];
+    for (int p0 = 0; p0 < kPasses; p0 += kAhead) {
+      Raw8<T> y[kAhead], z[kAhead];
 #pragma unroll
-      for (int p = p0; p < p0 + 2; ++p) {
-        const int r = p * kRowsPerPass + lane / kLanesPerRow;
+      for (int k = 0; k < kAhead; ++k) {
+        const int r = (p0 + k) * kRowsPerPass + r_lane;
         if (r >= lo && r < hi)
-          load_pair8(src + static_cast<long long>(e.tok0 + (blk * kBlock + r - row0)) * stride +
-                         h * HD, el, a.rope, kv == 0, x[p], z[p - p0]);
+          load_pair8(row_src + (p0 + k) * kRowsPerPass * stride, el, a.rope, kv == 0, y[k], z[k]);
       }
 #pragma unroll
-      for (int p = p0; p < p0 + 2; ++p) {
-        const int r = p * kRowsPerPass + lane / kLanesPerRow;
-        if (r >= lo && r < hi) {
-          if (kv == 0) rotate_pair8(el, a.rope, s_cs[r], x[p], z[p - p0]);
+      for (int k = 0; k < kAhead; ++k) {
+        const int p = p0 + k, r = p * kRowsPerPass + r_lane;
+        unpack8(y[k], x[p]);
+        if (r < lo || r >= hi) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) top = max(top, __float_as_uint(fabsf(x[p][j])));
+          for (int j = 0; j < 8; ++j) x[p][j] = 0.f;
+        } else if (kv == 0) {
+          float w[8];
+          unpack8(z[k], w);
+          rotate_pair8(el, a.rope, s_cs[r], x[p], w);
         }
+#pragma unroll
+        for (int j = 0; j < 8; j += 2) top = max3(top, fabsf(x[p][j]), fabsf(x[p][j + 1]));
+        // x - x is 0 but for NaN and infinity
+#pragma unroll
+        for (int j = 0; j < 8; ++j) odd |= __float_as_uint(__fsub_rn(x[p][j], x[p][j]));
       }
     }
-    top = __reduce_max_sync(0xffffffffu, top);
-    float s = __fdiv_rn(__uint_as_float(top), code_top<FMT>());
-    if (top >= 0x7f800000u) s = __uint_as_float(0x7fc00000u);
+    top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+    float s = __fdiv_rn(top, code_top<FMT>());
+    if (__any_sync(0xffffffffu, odd << 1)) s = __uint_as_float(0x7fc00000u);
     s = __uint_as_float(max(__float_as_uint(s), old_bits));
-    const Quotient over(s > 0.f ? s : 1.f);
+    const float by = s > 0.f ? s : 1.f;
+    const float inv = __fdiv_rn(1.f, by);
     const bool grown = lo > 0 && __float_as_uint(s) != old_bits;
-    const float ratio = s > 0.f ? __fdiv_rn(__uint_as_float(old_bits), s) : 1.f;
     __syncwarp();  // every lane has read the old scale
     if (lane == 0) *sc = s;
+    if (by > 1e-25f && by < 1e25f) {
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[p][j] = quotient(x[p][j], by, inv);
+    } else {
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll 1
+        for (int j = 0; j < 8; ++j) {
+          const float q = __fdiv_rn(x[p][0], by);  // in turn, to keep the code short
+#pragma unroll
+          for (int m = 0; m < 7; ++m) x[p][m] = x[p][m + 1];
+          x[p][7] = q;
+        }
+    }
 #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
-      const int r = p * kRowsPerPass + lane / kLanesPerRow;
-      uint2* at = reinterpret_cast<uint2*>(dst + r * HD);
-      if (r >= lo && r < hi) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[p][j] = over(x[p][j]);
-        *at = encode8<FMT>(x[p]);
-      } else if (r < lo && grown) {
+      const int r = p * kRowsPerPass + r_lane;
+      if (r >= lo && r < hi)
+        *reinterpret_cast<uint2*>(dst + r * HD) = encode8<FMT>(x[p]);
+    }
+    if (grown) {
+      const float ratio = s > 0.f ? __fdiv_rn(__uint_as_float(old_bits), s) : 1.f;
+#pragma unroll 1
+      for (int r = r_lane; r < lo; r += kRowsPerPass) {
+        uint2* at = reinterpret_cast<uint2*>(dst + r * HD);
         float y[8];
         decode8<FMT>(*at, y);
 #pragma unroll

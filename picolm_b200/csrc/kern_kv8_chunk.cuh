@@ -162,24 +162,6 @@ __device__ __forceinline__ float2 turn(float2 a, float2 b) {
   return make_float2(a.x * b.x - a.y * b.y, a.y * b.x + a.x * b.y);
 }
 
-// Eight elements as they are in memory.
-template <typename T>
-struct Raw8 {
-  uint4 v[sizeof(T) / 2];
-};
-template <typename T>
-__device__ __forceinline__ Raw8<T> raw8(const T* p) {
-  Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-    r.v[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-  return r;
-}
-template <typename T>
-__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&x)[8]) {
-  load8(reinterpret_cast<const T*>(r.v), x);
-}
-
 template <typename T, int HD, int FMT>
 __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
     const __grid_constant__ Kv8ChunkArgs ca) {

@@ -98,6 +98,24 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
   *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// Eight elements as they are in memory.
+template <typename T>
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> raw8(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
+    r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const Raw8<T>& r, float (&x)[8]) {
+  load8(reinterpret_cast<const T*>(r.v), x);
+}
+
 __device__ __forceinline__ float to_f32(float x) { return x; }
 __device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
 __device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
@@ -175,7 +193,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
 
 // Aligned rows.  A unit is eight elements of a head (LLaMA; past dim: copied)
 // or the two runs of eight that rotate together (Qwen, dim / 2 a multiple of
-// eight); a thread has the loads of four units under way.
+// eight).  A thread keeps its unit over the block's rows, so its place is
+// found once, and has the loads of four rows under way.
 template <typename T, bool LLAMA>
 __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
     const __grid_constant__ RopeRowsArgs a) {
@@ -184,61 +203,56 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
   const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
   const int row0 = blockIdx.x * a.rows_per_block;
   const int rows = min(a.rows_per_block, a.n - row0);
-  const int all = a.units;
+  const int u = blockIdx.y * kRopeThreads + threadIdx.x;
+  const bool mine = u < a.units;
+  const int h = static_cast<int>((static_cast<uint64_t>(u) * a.per_head_inv) >> 32);
+  const int c = u - h * a.per_head;
+  // Qwen: the runs below half, then those past dim
+  const int el = LLAMA || c * 8 < half ? c * 8 : c * 8 + half;
+  const bool two = !LLAMA && el < half, turns = el < a.rope.dim;
+  const bool is_q = h < a.n_heads;
+  const long long at = static_cast<long long>(is_q ? h : h - a.n_heads) * hd + el;
+  const long long in_step = is_q ? a.q_stride : a.k_stride;
+  const long long out_step = is_q ? a.qo_stride : a.ko_stride;
+  const T* src = static_cast<const T*>(is_q ? a.q : a.k) + row0 * in_step + at;
+  T* dst = static_cast<T*>(is_q ? a.qo : a.ko) + row0 * out_step + at;
   constexpr int U = 4;
-  const T* src[U];
-  T* dst[U];
-  int el[U], step = LLAMA ? 0 : half;  // from the first to the second run
-  float x[U][8], z[U][8];
-  // unit u of row r: its addresses; false past the row
-  auto find = [&](int u, int r, int k) {
-    const int h = static_cast<int>((static_cast<uint64_t>(u) * a.per_head_inv) >> 32);
-    const int c = u - h * a.per_head;
-    // Qwen: the runs below half, then those past dim
-    el[k] = LLAMA || c * 8 < half ? c * 8 : c * 8 + half;
-    const bool is_q = h < a.n_heads;
-    const long long row = row0 + r;
-    const long long at = static_cast<long long>(is_q ? h : h - a.n_heads) * hd + el[k];
-    src[k] = is_q ? static_cast<const T*>(a.q) + row * a.q_stride + at
-                  : static_cast<const T*>(a.k) + row * a.k_stride + at;
-    dst[k] = is_q ? static_cast<T*>(a.qo) + row * a.qo_stride + at
-                  : static_cast<T*>(a.ko) + row * a.ko_stride + at;
+  Raw8<T> x[U], z[U];
+  auto fetch = [&](int r0) {
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (mine && r0 + k < rows) {
+        x[k] = raw8(src + (r0 + k) * in_step);
+        if (two) z[k] = raw8(src + (r0 + k) * in_step + half);
+      }
   };
-  auto rotate = [&](int r, int k) {
-    const float2* cs = s_cs[r];
-    if constexpr (LLAMA) {
+  fetch(0);  // on their way while the cosines are computed
+  rope_rows_table(a, row0, rows, s_cs, s_turns);
+#pragma unroll 1
+  for (int r0 = 0; r0 < rows; r0 += U) {
+    if (r0) fetch(r0);
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (el[k] + 2 * i < a.rope.dim)
-          rope_one(x[k][2 * i], x[k][2 * i + 1], cs[(el[k] >> 1) + i]);
-    } else if (el[k] < half) {
+    for (int k = 0; k < U; ++k) {
+      if (!mine || r0 + k >= rows) break;
+      float y[8];
+      unpack8(x[k], y);
+      const float2* cs = s_cs[r0 + k];
+      if constexpr (LLAMA) {
+        if (turns) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) rope_one(x[k][i], z[k][i], cs[el[k] + i]);
-      store8(dst[k] + step, z[k]);
-    }
-    store8(dst[k], x[k]);
-  };
-  // the first units are on their way while the cosines are computed
-  bool first = true;
-  for (int r = 0; r < rows; ++r)
-    for (int u0 = threadIdx.x; u0 < all || first; u0 += U * kRopeThreads) {
-#pragma unroll
-      for (int k = 0; k < U; ++k) {
-        const int u = u0 + k * kRopeThreads;
-        if (u < all) {
-          find(u, r, k);
-          load8(src[k], x[k]);
-          if (!LLAMA && el[k] < half) load8(src[k] + step, z[k]);
+          for (int i = 0; i < 4; ++i)
+            if (el + 2 * i < a.rope.dim) rope_one(y[2 * i], y[2 * i + 1], cs[(el >> 1) + i]);
         }
-      }
-      if (first) {
-        rope_rows_table(a, row0, rows, s_cs, s_turns);
-        first = false;
-      }
+      } else if (two) {
+        float w[8];
+        unpack8(z[k], w);
 #pragma unroll
-      for (int k = 0; k < U; ++k)
-        if (u0 + k * kRopeThreads < all) rotate(r, k);
+        for (int i = 0; i < 8; ++i) rope_one(y[i], w[i], cs[el + i]);
+        store8(dst + (r0 + k) * out_step + half, w);
+      }
+      store8(dst + (r0 + k) * out_step, y);
     }
+  }
 }
 
 }  // namespace pl

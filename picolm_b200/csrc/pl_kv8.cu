@@ -450,9 +450,10 @@ int pl_rope_rows_dev(const pl_rope* r, int dtype, int n, const int* d_pos, int n
   a.per_head = llama ? r->head_dim / 8 : half / 8 + (r->head_dim - r->dim) / 8;
   a.units = a.per_head * (n_heads + n_kv_heads);
   a.per_head_inv = fast ? ((1ull << 32) + a.per_head - 1) / a.per_head : 0;
+  const dim3 grid_vec(grid.x, (a.units + pl::kRopeThreads - 1) / pl::kRopeThreads);
   auto go = [&](auto any, auto by_pairs, auto by_halves) {
-    return launch(!fast ? any : llama ? by_pairs : by_halves, grid, pl::kRopeThreads, 0, stream,
-                  false, a);
+    return launch(!fast ? any : llama ? by_pairs : by_halves, fast ? grid_vec : grid,
+                  pl::kRopeThreads, 0, stream, false, a);
   };
   if (dtype == PL_F32)
     return go(pl::rope_rows_any_kernel<float>, pl::rope_rows_kernel<float, true>,
