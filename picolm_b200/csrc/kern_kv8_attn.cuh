@@ -235,6 +235,18 @@ __device__ __forceinline__ uint32_t tile_off(int r, int ch) {
   return r * 128 + ((ch ^ (r & 7)) << 4);
 }
 
+// Counts one arrival at a counter in global memory: what the warp (or block)
+// wrote before, ordered by its own barrier, is visible to who counts later,
+// and what earlier arrivals wrote to this thread.
+__device__ __forceinline__ int arrive_acq_rel(int* counter) {
+  int old;
+  asm volatile("atom.add.acq_rel.gpu.global.s32 %0, [%1], 1;"
+               : "=r"(old)
+               : "l"(counter)
+               : "memory");
+  return old;
+}
+
 // The list of tiles: prefix sums over entries, in tiles of all heads.
 template <int HD>
 struct DecWork {
@@ -249,7 +261,13 @@ struct DecWork {
     return static_cast<int>(((static_cast<long long>(x) + 1) * blocks - 1) / total);
   }
   __device__ __forceinline__ int entry_of(int x) const {
-    int lo = 0, hi = n - 1;
+    // right at once where the entries are alike
+    int lo = static_cast<int>(static_cast<float>(x) * (static_cast<float>(n) /
+                                                       static_cast<float>(total)));
+    lo = min(lo, n - 1);
+    if (prefix[lo] <= x && x < prefix[lo + 1]) return lo;
+    lo = 0;
+    int hi = n - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
       if (prefix[mid + 1] > x) hi = mid; else lo = mid + 1;
@@ -494,8 +512,7 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
       const int s = (x - x0) % NS;
       uint64_t* bar = &sm.full[warp][s];
       mbar_arrive_expect_tx(bar, 2 * Sh::kTileBytes + 2 * kBlocksPerPage * 4);
-      tma_load_3d(sm.ring[warp][s][0], &tm, bar, 0, row % kPage, slab);
-      tma_load_3d(sm.ring[warp][s][1], &tm, bar, 0, row % kPage, slab + 1);
+      tma_load_3d(sm.ring[warp][s][0], &tm, bar, 0, row % kPage, slab);  // K and V
       bulk_load(sm.scales[warp][s], a.g.scales + static_cast<long long>(slab) * kBlocksPerPage,
                 2 * kBlocksPerPage * 4, bar);
     }
@@ -758,16 +775,14 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
   // more of them with all warps below.
   auto publish = [&](int r, int first, int last, int kind) {
     st.save(da.part + static_cast<long long>(2 * blk + kind) * Sh::kPartFloats, lane);
-    __threadfence();
-    __syncwarp();
     const int f0 = work.block_of(first), parts = work.block_of(last) - f0 + 1;
+    __syncwarp();
     int done = 0;
     if (lane == 0) {
-      done = atomicAdd(&da.arrived[f0], 1) == parts - 1;
+      done = arrive_acq_rel(&da.arrived[f0]) == parts - 1;
       if (done) {
         da.arrived[f0] = 0;
         if (parts > 4) sm.finish[kind] = r;
-        __threadfence();
       }
     }
     done = __shfl_sync(0xffffffffu, done, 0);

@@ -86,7 +86,8 @@ int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
 }
 
 // The codes as [slab][64 rows][head_dim] bytes, slab = (page, layer, head,
-// K or V), read in boxes of `rows` rows under the swizzle of a row's width.
+// K or V), read in boxes of `rows` rows of K and V under the swizzle of a
+// row's width.
 int codes_map(const pl_kv8* c, int rows, CUtensorMap* m) {
   typedef CUresult (*EncodeFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
                                const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -109,7 +110,7 @@ int codes_map(const pl_kv8* c, int rows, CUtensorMap* m) {
       hd, PL_KV8_PAGE,
       static_cast<cuuint64_t>(c->n_pages) * c->n_layers * c->n_kv_heads * 2};
   const cuuint64_t strides[2] = {hd, hd * PL_KV8_PAGE};
-  const cuuint32_t box[3] = {static_cast<cuuint32_t>(hd), static_cast<cuuint32_t>(rows), 1u};
+  const cuuint32_t box[3] = {static_cast<cuuint32_t>(hd), static_cast<cuuint32_t>(rows), 2u};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r =
       fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c->codes, dims, strides, box, estr,
