@@ -175,6 +175,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int heads = a.g.n_kv_heads, G = a.group;
   const int slot_tok = kChRows / G, per_item = 2 * slot_tok;
+  const uint32_t inv_g = (65536 + G - 1) / G;  // r / G = r * inv_g >> 16 for a slot's rows
+  // Place of pair i in a table of cosines: the pairs that the lanes of a row
+  // want at once (every fourth or eighth) lie side by side.
+  const int pair_log = a.rope.type == PL_ROPE_LLAMA ? 2 : 3;
+  auto place = [&](int i) {
+    return (i & ((1 << pair_log) - 1)) * ((HD / 2) >> pair_log) + (i >> pair_log);
+  };
   uint32_t* err = &a.g.head->err;
 
   if (tid < HD / 2) sm.half_turns[tid] = a.rope.half_turns[tid];
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
   __syncthreads();  // half_turns
   for (int t = tid; t < 24 * (HD / 2); t += kChThreads) {
     const int w = t / (HD / 2), i = t % (HD / 2);
-    sm.step[w][i] = rope_cs_fast(sm.half_turns[i], 1.0, w < 8 ? w : 8 * (w - 8));
+    sm.step[w][place(i)] = rope_cs_fast(sm.half_turns[i], 1.0, w < 8 ? w : 8 * (w - 8));
   }
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -558,7 +565,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
     // -------------------------------------------------------------- softmax
     const int x = warp >> 2;        // slot
     const int r = tid & 127;        // query row of the slot, TMEM lane
-    const int row_tok = r / G, row_head = r - row_tok * G;
+    const int row_tok = r * inv_g >> 16, row_head = r - row_tok * G;
     const uint32_t lane_base = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     int J = 0, A = 0, n_merge = 0;
     // a wait that gave up ends this warp's arithmetic; it still takes its
@@ -588,16 +595,17 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         const int e = (lane % LR) * 8, half = a.rope.dim >> 1;
         const bool llama = a.rope.type == PL_ROPE_LLAMA;
         for (int i = lane; i < half; i += 32)
-          sm.base[warp][i] = rope_cs_fast(sm.half_turns[i], a.rope.gain, p_min);
+          sm.base[warp][place(i)] = rope_cs_fast(sm.half_turns[i], a.rope.gain, p_min);
         __syncwarp();
         auto row_at = [&](int it) { return (warp & 3) * 32 + it * RI + lane / LR; };
+        const int n_tok = g.n_tok;
+        const T* q_slot = static_cast<const T*>(a.q) +
+                          (static_cast<long long>(g.tok0) + tok_x) * a.q_stride + g.h * G * HD;
         auto q_row = [&](int row, bool& there) -> const T* {
-          const int tk = row / G;
-          there = tk < slot_tok && tok_x + tk < g.n_tok;
+          const int tk = row * inv_g >> 16;
+          there = tk < slot_tok && tok_x + tk < n_tok;
           if (!there) return static_cast<const T*>(a.q);
-          return static_cast<const T*>(a.q) +
-                 (static_cast<long long>(g.tok0) + tok_x + tk) * a.q_stride +
-                 (g.h * G + row - tk * G) * HD;
+          return q_slot + tk * a.q_stride + (row - tk * G) * HD;
         };
         // four rows ahead; the loop is not unrolled, because it runs once a
         // segment and fetching the unrolled code took longer than running it
@@ -609,7 +617,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         int cs_tok = -1;
 #pragma unroll 1
         for (int it = 0; it < LR; ++it) {
-          const int row = row_at(it), tk = row / G;
+          const int row = row_at(it), tk = row * inv_g >> 16;
           float y[8];
           unpack8(raw[0], y);
 #pragma unroll
@@ -627,7 +635,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
             for (int d = 0; d < 8; ++d) {
               const int el = e + d;
               if (llama && (d & 1)) continue;
-              const int i = llama ? el >> 1 : el < half ? el : el - half;
+              const int i = place(llama ? el >> 1 : el < half ? el : el - half);
               if (el < a.rope.dim)
                 f[d] = turn(turn(sm.base[warp][i], sm.step[8 + (tt >> 3)][i]), sm.step[tt & 7][i]);
             }
@@ -641,16 +649,23 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
                 y[d + 1] = u * f[d].y + v * f[d].x;
               }
           } else {
-            const bool lanes = a.rope.dim == HD;  // the partner is in another lane, or in memory
+            float o[8];  // the partners: in another lane, or in memory
+            if (a.rope.dim == HD) {
 #pragma unroll
-            for (int d = 0; d < 8; ++d) {
-              const int el = e + d;
-              float o = __shfl_xor_sync(0xffffffffu, y[d], LR / 2);
-              if (!lanes && there && el < a.rope.dim)
-                o = to_f32(q[el < half ? el + half : el - half]);
-              if (el < a.rope.dim)
-                y[d] = el < half ? y[d] * f[d].x - o * f[d].y : o * f[d].y + y[d] * f[d].x;
+              for (int d = 0; d < 8; ++d) o[d] = __shfl_xor_sync(0xffffffffu, y[d], LR / 2);
+            } else {
+#pragma unroll
+              for (int d = 0; d < 8; ++d) {
+                const int el = e + d;
+                o[d] = there && el < a.rope.dim ? to_f32(q[el < half ? el + half : el - half]) : 0.f;
+              }
             }
+#pragma unroll
+            for (int d = 0; d < 8; ++d)
+              if (e + d < a.rope.dim) {
+                const float s = e + d < half ? -f[d].y : f[d].y;
+                y[d] = fmaf(y[d], f[d].x, o[d] * s);
+              }
           }
           float top = 0.f;
 #pragma unroll
