@@ -156,7 +156,8 @@ __device__ __forceinline__ void load_pair8(const T* x, int e, const pl_rope& r, 
     }
   }
 }
-// y rotated by cs[pair], with the roundings of rope().
+// y rotated by cs[place of the pair], with the roundings of rope().
+template <int HD>
 __device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const float2* cs,
                                              float (&y)[8], const float (&z)[8]) {
   if (e >= r.dim) return;
@@ -164,15 +165,15 @@ __device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const floa
   if (r.type == PL_ROPE_LLAMA) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (e + 2 * j < r.dim) rope_one(y[2 * j], y[2 * j + 1], cs[(e >> 1) + j]);
+      if (e + 2 * j < r.dim) rope_one(y[2 * j], y[2 * j + 1], cs[pair_place<true>((e >> 1) + j, HD / 2)]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int d = e + j;
-      if (d < half)
-        y[j] = __fsub_rn(__fmul_rn(y[j], cs[d].x), __fmul_rn(z[j], cs[d].y));
-      else if (d < r.dim)
-        y[j] = __fadd_rn(__fmul_rn(z[j], cs[d - half].y), __fmul_rn(y[j], cs[d - half].x));
+      if (d >= r.dim) break;
+      const float2 f = cs[pair_place<false>(d < half ? d : d - half, HD / 2)];
+      y[j] = d < half ? __fsub_rn(__fmul_rn(y[j], f.x), __fmul_rn(z[j], f.y))
+                      : __fadd_rn(__fmul_rn(z[j], f.y), __fmul_rn(y[j], f.x));
     }
   }
 }
@@ -232,8 +233,10 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
       double s, c, ss = 0.0, sc = 1.0;
       sincospi(s_turns[i] * static_cast<double>(blk * kBlock + r0), &s, &c);
       if (r1 - r0 > 1) sincospi(s_turns[i], &ss, &sc);
+      const int at = a.rope.type == PL_ROPE_LLAMA ? pair_place<true>(i, HD / 2)
+                                                  : pair_place<false>(i, HD / 2);
       for (int r = r0; r < r1; ++r) {
-        s_cs[r][i] = make_float2(static_cast<float>(c * a.rope.gain),
+        s_cs[r][at] = make_float2(static_cast<float>(c * a.rope.gain),
                                  static_cast<float>(s * a.rope.gain));
         const double nc = c * sc - s * ss;
         s = s * sc + c * ss;
@@ -280,7 +283,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
         } else if (kv == 0) {
           float w[8];
           unpack8(z[k], w);
-          rotate_pair8(el, a.rope, s_cs[r], x[p], w);
+          rotate_pair8<HD>(el, a.rope, s_cs[r], x[p], w);
         }
 #pragma unroll
         for (int j = 0; j < 8; j += 2) top = max3(top, fabsf(x[p][j]), fabsf(x[p][j + 1]));

@@ -134,7 +134,17 @@ struct RopeRowsArgs {
   long long q_stride, qo_stride, k_stride, ko_stride;  // elements between rows
 };
 
+// Place of pair i in a table of n (a multiple of 8) pairs.  Neighbouring lanes
+// rotate neighbouring runs of eight elements, four pairs (LLaMA) or eight
+// (Qwen) apart: what they read together lies side by side here, free of
+// bank conflicts.
+template <bool LLAMA>
+__device__ __forceinline__ int pair_place(int i, int n) {
+  return LLAMA ? (i & 3) * (n / 4) + (i >> 2) : (i & 7) * (n / 8) + (i >> 3);
+}
+
 // Cosines and sines of the block's rows, once for all heads.
+template <bool LLAMA>
 __device__ __forceinline__ void rope_rows_table(const RopeRowsArgs& a, int row0, int rows,
                                                 float2 (*s_cs)[PL_ROPE_MAX_PAIRS],
                                                 double* s_turns) {
@@ -145,7 +155,7 @@ __device__ __forceinline__ void rope_rows_table(const RopeRowsArgs& a, int row0,
     const int r = t / half, i = t - r * half;
     float2 cs = rope_cs(s_turns[i], a.rope.gain, a.pos[row0 + r]);
     if (a.adjoint) cs.y = -cs.y;
-    s_cs[r][i] = cs;
+    s_cs[r][pair_place<LLAMA>(i, PL_ROPE_MAX_PAIRS)] = cs;
   }
   __syncthreads();
 }
@@ -167,7 +177,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
   const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
   const int row0 = blockIdx.x * a.rows_per_block;
   const int rows = min(a.rows_per_block, a.n - row0);
-  rope_rows_table(a, row0, rows, s_cs, s_turns);
+  rope_rows_table<true>(a, row0, rows, s_cs, s_turns);
   const int heads = a.n_heads + a.n_kv_heads;
   const int per_head = half + (hd - a.rope.dim);
   for (int t = threadIdx.x; t < rows * heads * per_head; t += kRopeThreads) {
@@ -182,7 +192,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
       const bool llama = a.rope.type == PL_ROPE_LLAMA;
       const int ea = llama ? 2 * u : u, eb = llama ? 2 * u + 1 : u + half;
       float xa = to_f32(x[ea]), xb = to_f32(x[eb]);
-      rope_one(xa, xb, s_cs[r][u]);
+      rope_one(xa, xb, s_cs[r][pair_place<true>(u, PL_ROPE_MAX_PAIRS)]);
       from_f32(y + ea, xa);
       from_f32(y + eb, xb);
     } else {
@@ -227,7 +237,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
       }
   };
   fetch(0);  // on their way while the cosines are computed
-  rope_rows_table(a, row0, rows, s_cs, s_turns);
+  rope_rows_table<LLAMA>(a, row0, rows, s_cs, s_turns);
 #pragma unroll 1
   for (int r0 = 0; r0 < rows; r0 += U) {
     if (r0) fetch(r0);
@@ -241,13 +251,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
         if (turns) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (el + 2 * i < a.rope.dim) rope_one(y[2 * i], y[2 * i + 1], cs[(el >> 1) + i]);
+            if (el + 2 * i < a.rope.dim) rope_one(y[2 * i], y[2 * i + 1],
+                       cs[pair_place<true>((el >> 1) + i, PL_ROPE_MAX_PAIRS)]);
         }
       } else if (two) {
         float w[8];
         unpack8(z[k], w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rope_one(y[i], w[i], cs[el + i]);
+        for (int i = 0; i < 8; ++i) rope_one(y[i], w[i], cs[pair_place<false>(el + i, PL_ROPE_MAX_PAIRS)]);
         store8(dst + (r0 + k) * out_step + half, w);
       }
       store8(dst + (r0 + k) * out_step, y);
