@@ -199,10 +199,11 @@ __device__ __forceinline__ float quotient(float x, float by, float inv) {
 // row was appended; a block of rows takes two sincospi a pair (its first
 // row's and one row's step) and turns from row to row by FP64 products.
 template <typename T, int HD, int FMT>
-__global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
+__global__ void __launch_bounds__(kAppendThreads, 3) kv8_append_kernel(
     const __grid_constant__ Kv8AppendArgs a) {
   __shared__ float2 s_cs[kBlock][HD / 2];
   __shared__ double s_turns[HD / 2];
+  __shared__ uint32_t s_top[2][kAppendThreads / 32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x < HD / 2) s_turns[threadIdx.x] = a.rope.half_turns[threadIdx.x];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -245,11 +246,17 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
     }
   }
   __syncthreads();
+  // HD / 64 warps share a (head, K or V), so that no warp holds more than
+  // 32 values a lane
   constexpr int kLanesPerRow = HD / 8, kRowsPerPass = 32 / kLanesPerRow;
-  constexpr int kPasses = kBlock / kRowsPerPass;
+  constexpr int kSplit = HD / 64, kRowsPerWarp = kBlock / kSplit;
+  constexpr int kPasses = kRowsPerWarp / kRowsPerPass;
+  constexpr int kTeams = kAppendThreads / 32 / kSplit;
+  const int team = warp / kSplit, row_first = warp % kSplit * kRowsPerWarp;
   const int el = (lane % kLanesPerRow) * 8;
   const int sub = blk % kBlocksPerPage;
-  for (int u = warp; u < 2 * a.g.n_kv_heads; u += kAppendThreads / 32) {
+  int turn = 0;
+  for (int u = team; u < 2 * a.g.n_kv_heads; u += kTeams) {
     const int h = u >> 1, kv = u & 1;
     const long long slab = a.g.slab(page, h, kv);
     uint8_t* dst = a.g.codes + (slab * kPage + sub * kBlock) * HD + el;
@@ -260,10 +267,10 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
     float x[kPasses][8];
     float top = 0.f;
     uint32_t odd = 0;  // a NaN or infinity
+    const int r_lane = row_first + lane / kLanesPerRow;
     const T* row_src = src + static_cast<long long>(e.tok0 + (blk * kBlock - row0) +
-                                                    lane / kLanesPerRow) * stride + h * HD;
-    const int r_lane = lane / kLanesPerRow;
-    constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // rows under way
+                                                    r_lane) * stride + h * HD;
+    constexpr int kAhead = sizeof(T) == 4 ? 1 : 2;  // rows under way
 #pragma unroll
     for (int p0 = 0; p0 < kPasses; p0 += kAhead) {
       Raw8<T> y[kAhead], z[kAhead];
@@ -293,14 +300,23 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
       }
     }
     top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
-    float s = __fdiv_rn(top, code_top<FMT>());
-    if (__any_sync(0xffffffffu, odd << 1)) s = __uint_as_float(0x7fc00000u);
+    if (__any_sync(0xffffffffu, odd << 1)) top = __uint_as_float(0x7fc00000u);
+    if constexpr (kSplit > 1) {
+      if (lane == 0) s_top[turn][warp] = __float_as_uint(top);
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "r"(32 * kSplit) : "memory");
+#pragma unroll
+      for (int w = 0; w < kSplit; ++w)
+        top = __uint_as_float(max(__float_as_uint(top), s_top[turn][team * kSplit + w]));
+      turn ^= 1;
+    }
+    float s = top;
+    if (__float_as_uint(top) <= 0x7f800000u) s = __fdiv_rn(top, code_top<FMT>());
     s = __uint_as_float(max(__float_as_uint(s), old_bits));
     const float by = s > 0.f ? s : 1.f;
     const float inv = __fdiv_rn(1.f, by);
     const bool grown = lo > 0 && __float_as_uint(s) != old_bits;
     __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *sc = s;
+    if (lane == 0 && row_first == 0) *sc = s;
     if (by > 1e-25f && by < 1e25f) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)
@@ -326,7 +342,7 @@ __global__ void __launch_bounds__(kAppendThreads, 2) kv8_append_kernel(
     if (grown) {
       const float ratio = s > 0.f ? __fdiv_rn(__uint_as_float(old_bits), s) : 1.f;
 #pragma unroll 1
-      for (int r = r_lane; r < lo; r += kRowsPerPass) {
+      for (int r = r_lane; r < min(lo, row_first + kRowsPerWarp); r += kRowsPerPass) {
         uint2* at = reinterpret_cast<uint2*>(dst + r * HD);
         float y[8];
         decode8<FMT>(*at, y);

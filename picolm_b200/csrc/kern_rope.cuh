@@ -22,7 +22,7 @@
 
 namespace pl {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 256;  // at most
 constexpr int kRopeRows = 8;  // rows per block, at most
 
 // Cosine and sine of a pair at position pos, times the gain, rounded once
@@ -149,9 +149,9 @@ __device__ __forceinline__ void rope_rows_table(const RopeRowsArgs& a, int row0,
                                                 float2 (*s_cs)[PL_ROPE_MAX_PAIRS],
                                                 double* s_turns) {
   const int half = a.rope.dim >> 1;
-  for (int i = threadIdx.x; i < half; i += kRopeThreads) s_turns[i] = a.rope.half_turns[i];
+  for (int i = threadIdx.x; i < half; i += blockDim.x) s_turns[i] = a.rope.half_turns[i];
   __syncthreads();
-  for (int t = threadIdx.x; t < rows * half; t += kRopeThreads) {
+  for (int t = threadIdx.x; t < rows * half; t += blockDim.x) {
     const int r = t / half, i = t - r * half;
     float2 cs = rope_cs(s_turns[i], a.rope.gain, a.pos[row0 + r]);
     if (a.adjoint) cs.y = -cs.y;
@@ -206,14 +206,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
 // eight).  A thread keeps its unit over the block's rows, so its place is
 // found once, and has the loads of four rows under way.
 template <typename T, bool LLAMA>
-__global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
+__global__ void __launch_bounds__(kRopeThreads, sizeof(T) == 4 ? 2 : 3) rope_rows_kernel(
     const __grid_constant__ RopeRowsArgs a) {
   __shared__ float2 s_cs[kRopeRows][PL_ROPE_MAX_PAIRS];
   __shared__ double s_turns[PL_ROPE_MAX_PAIRS];
   const int hd = a.rope.head_dim, half = a.rope.dim >> 1;
   const int row0 = blockIdx.x * a.rows_per_block;
   const int rows = min(a.rows_per_block, a.n - row0);
-  const int u = blockIdx.y * kRopeThreads + threadIdx.x;
+  const int u = blockIdx.y * blockDim.x + threadIdx.x;
   const bool mine = u < a.units;
   const int h = static_cast<int>((static_cast<uint64_t>(u) * a.per_head_inv) >> 32);
   const int c = u - h * a.per_head;
@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_kernel(
   const long long out_step = is_q ? a.qo_stride : a.ko_stride;
   const T* src = static_cast<const T*>(is_q ? a.q : a.k) + row0 * in_step + at;
   T* dst = static_cast<T*>(is_q ? a.qo : a.ko) + row0 * out_step + at;
-  constexpr int U = 4;
+  constexpr int U = LLAMA ? 4 : 2;
   Raw8<T> x[U], z[U];
   auto fetch = [&](int r0) {
 #pragma unroll

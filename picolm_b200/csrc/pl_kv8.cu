@@ -451,10 +451,13 @@ int pl_rope_rows_dev(const pl_rope* r, int dtype, int n, const int* d_pos, int n
   a.per_head = llama ? r->head_dim / 8 : half / 8 + (r->head_dim - r->dim) / 8;
   a.units = a.per_head * (n_heads + n_kv_heads);
   a.per_head_inv = fast ? ((1ull << 32) + a.per_head - 1) / a.per_head : 0;
-  const dim3 grid_vec(grid.x, (a.units + pl::kRopeThreads - 1) / pl::kRopeThreads);
+  // blocks of equal width along a row
+  const int across = (a.units + pl::kRopeThreads - 1) / pl::kRopeThreads;
+  const int width = fast ? ((a.units + across - 1) / across + 31) / 32 * 32 : pl::kRopeThreads;
+  const dim3 grid_vec(grid.x, across);
   auto go = [&](auto any, auto by_pairs, auto by_halves) {
     return launch(!fast ? any : llama ? by_pairs : by_halves, fast ? grid_vec : grid,
-                  pl::kRopeThreads, 0, stream, false, a);
+                  width, 0, stream, false, a);
   };
   if (dtype == PL_F32)
     return go(pl::rope_rows_any_kernel<float>, pl::rope_rows_kernel<float, true>,
