@@ -457,8 +457,13 @@ int  pl_rope_rows_dev(const pl_rope *r, int dtype, int n, const int *d_pos,
  * ordered by the caller.  Different caches are independent.  The current
  * device must be the cache's (PL_EDEVICE).  Arrays of a call are device
  * memory; a slot, row count or page out of range that a kernel finds there
- * leaves its entry (its call, for the page operations) undone and is
- * reported by pl_kv8_status as PL_EARG.  Slots of one call are distinct.
+ * leaves its entry (its call, for the page operations) undone, or the entry's
+ * output undefined where attention has begun, and is reported by
+ * pl_kv8_status as PL_EARG.  Slots of one call are distinct wherever it
+ * writes to the cache or its books; attention and read-back may name one
+ * several times.  The bound on device-side waits is pl_attn_set_wait_limit's
+ * (2 s without a context).  A call has n <= 1024 entries, and fewer than
+ * 2^29 / (max_pages * n_kv_heads) (PL_EARG).
  * Inputs and outputs are `dtype` rows of heads x head_dim elements, 16-byte
  * aligned with strides (in elements) that are multiples of 16 bytes. */
 /* Bytes of the workspace of a cache of this shape. */

@@ -10,8 +10,8 @@ through cudaGetDriverEntryPoint, so the library has no link-time dependency
 on libcuda and loads on a host without a GPU (its calls then fail with
 PL_EDEVICE).  ptxas' resource report (registers, spills per kernel) is
 kept beside the library in libpl_attn.resources.json, and the build fails if
-the prefill kernels do not have the register count their warpgroup split
-needs.
+the kernels that split their registers between warpgroups do not have the
+count the split needs.
 """
 from __future__ import annotations
 
@@ -65,6 +65,8 @@ RESOURCES = os.path.join(HERE, "libpl_attn.resources.json")
 # launch (65536 / 384 threads, rounded down to 8), or the increase of the
 # softmax warpgroups can never be granted.
 PREFILL_LAUNCH_REGS = 168
+# The same for the 8-bit cache's chunk attention: 65536 / 512 threads.
+CHUNK_LAUNCH_REGS = 128
 
 
 def parse_ptxas(text: str) -> dict:
@@ -92,14 +94,15 @@ def parse_ptxas(text: str) -> dict:
 def check_resources(res: dict) -> None:
     """Fail the build, not a later launch, when a toolkit change moves the
     prefill kernels off the register count their warpgroup split needs."""
-    pf = {k: v for k, v in res.items() if "prefill_attn_kernel" in k}
-    if not pf:
-        raise RuntimeError("ptxas reported no prefill_attn_kernel")
-    bad = {k: v.get("registers") for k, v in pf.items()
-           if v.get("registers") != PREFILL_LAUNCH_REGS}
-    if bad:
-        raise RuntimeError(f"prefill kernels need {PREFILL_LAUNCH_REGS} registers per thread "
-                           f"at launch, ptxas gave {bad}")
+    for name, regs in (("prefill_attn_kernel", PREFILL_LAUNCH_REGS),
+                       ("kv8_chunk_kernel", CHUNK_LAUNCH_REGS)):
+        of = {k: v for k, v in res.items() if name in k}
+        if not of:
+            raise RuntimeError(f"ptxas reported no {name}")
+        bad = {k: v.get("registers") for k, v in of.items() if v.get("registers") != regs}
+        if bad:
+            raise RuntimeError(f"{name} needs {regs} registers per thread at launch, "
+                               f"ptxas gave {bad}")
 
 
 def build(force: bool = False, verbose: bool = False) -> str:

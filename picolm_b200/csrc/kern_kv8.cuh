@@ -165,7 +165,8 @@ __device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const floa
   if (r.type == PL_ROPE_LLAMA) {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (e + 2 * j < r.dim) rope_one(y[2 * j], y[2 * j + 1], cs[pair_place<true>((e >> 1) + j, HD / 2)]);
+      if (e + 2 * j < r.dim)
+        rope_one(y[2 * j], y[2 * j + 1], cs[pair_place<true>((e >> 1) + j, HD / 2)]);
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j) {

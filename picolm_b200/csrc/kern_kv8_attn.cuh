@@ -207,26 +207,6 @@ __device__ __forceinline__ uint32_t codes_half2(uint32_t w) {
   }
 }
 
-// The same, e4m3 by its bits: sign, exponent and mantissa moved to their
-// places in FP16 are the code over 2^8 (subnormals too), exactly.  The
-// conversion instruction shares its unit with 2^x.
-template <int FMT, int SEL>
-__device__ __forceinline__ uint32_t codes_bits2(uint32_t w) {
-  if constexpr (FMT == PL_KV8_INT8) {
-    return codes_half2<FMT, SEL>(w);
-  } else {
-    // bytes a, b of w to the upper bytes of the halves
-    constexpr uint32_t sel = 4u | ((SEL & 0xf) << 4) | (4u << 8) | ((SEL >> 4) << 12);
-    const uint32_t t = __byte_perm(w, 0u, sel);
-    return (t & 0x80008000u) | ((t >> 1) & 0x3f803f80u);
-  }
-}
-// What codes_bits2 divides a code by.
-template <int FMT>
-__device__ __forceinline__ float code_unit() {
-  return FMT == PL_KV8_INT8 ? 1.f : 256.f;
-}
-
 // Byte offset of 16-byte chunk `ch` of row r in a tile of HD-byte rows, as
 // the TMA swizzle of that width places it.
 template <int HD>

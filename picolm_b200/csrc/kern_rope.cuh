@@ -32,9 +32,6 @@ __device__ __forceinline__ float2 rope_cs(double half_turns, double gain, int po
   sincospi(half_turns * static_cast<double>(pos), &s, &c);
   return make_float2(static_cast<float>(c * gain), static_cast<float>(s * gain));
 }
-__device__ __forceinline__ float2 rope_cs(const pl_rope& r, int i, int pos) {
-  return rope_cs(r.half_turns[i], r.gain, pos);
-}
 
 // The same in FP32 after an exact reduction to [-1, 1] half turns in FP64:
 // within 2e-7 of rope_cs, at a tenth of its time.  For q, which no rounding
@@ -45,9 +42,6 @@ __device__ __forceinline__ float2 rope_cs_fast(double half_turns, double gain, i
   sincospif(static_cast<float>(x - 2.0 * rint(0.5 * x)), &s, &c);
   const float g = static_cast<float>(gain);
   return make_float2(c * g, s * g);
-}
-__device__ __forceinline__ float2 rope_cs_fast(const pl_rope& r, int i, int pos) {
-  return rope_cs_fast(r.half_turns[i], r.gain, pos);
 }
 
 // Eight consecutive elements as FP32 (16-byte aligned FP16 / BF16, 32-byte
@@ -251,14 +245,16 @@ __global__ void __launch_bounds__(kRopeThreads, sizeof(T) == 4 ? 2 : 3) rope_row
         if (turns) {
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            if (el + 2 * i < a.rope.dim) rope_one(y[2 * i], y[2 * i + 1],
+            if (el + 2 * i < a.rope.dim)
+              rope_one(y[2 * i], y[2 * i + 1],
                        cs[pair_place<true>((el >> 1) + i, PL_ROPE_MAX_PAIRS)]);
         }
       } else if (two) {
         float w[8];
         unpack8(z[k], w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) rope_one(y[i], w[i], cs[pair_place<false>(el + i, PL_ROPE_MAX_PAIRS)]);
+        for (int i = 0; i < 8; ++i)
+          rope_one(y[i], w[i], cs[pair_place<false>(el + i, PL_ROPE_MAX_PAIRS)]);
         store8(dst + (r0 + k) * out_step + half, w);
       }
       store8(dst + (r0 + k) * out_step, y);

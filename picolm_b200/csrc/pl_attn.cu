@@ -892,6 +892,7 @@ int create_ctx(int n_layers, int n_heads, int n_kv_heads, int head_dim, int rope
     const uint64_t ns = pl::kDefaultWaitLimitNs;
     cudaMemcpyToSymbolAsync(pl::g_wait_limit_ns, &ns, sizeof(ns), 0, cudaMemcpyHostToDevice,
                             c->stream);
+    pl_module::kv8_wait_limit(ns);
   }
   {
     const size_t n = static_cast<size_t>(rope_rows) * (head_dim / 2);
@@ -1634,6 +1635,7 @@ int pl_attn_set_wait_limit(double seconds) {
   if (g_multi) return multi_set_wait_limit(ns);
   if (cudaSetDevice(g->device) != cudaSuccess) return PL_ECUDA;
   PL_CUDA(cudaMemcpyToSymbol(pl::g_wait_limit_ns, &ns, sizeof(ns)));
+  PL_CUDA(pl_module::kv8_wait_limit(ns));
   return PL_OK;
 }
 
@@ -2608,6 +2610,7 @@ int multi_set_wait_limit(uint64_t ns) {
   for (Ctx* c : g_multi->devs) {
     UseCtx u(c);
     PL_CUDA(cudaMemcpyToSymbol(pl::g_wait_limit_ns, &ns, sizeof(ns)));
+    PL_CUDA(pl_module::kv8_wait_limit(ns));
   }
   return PL_OK;
 }

@@ -16,6 +16,14 @@
 #include "kern_rope.cuh"
 #include "pl_kv8.h"
 
+namespace pl_module {
+
+cudaError_t kv8_wait_limit(uint64_t ns) {
+  return cudaMemcpyToSymbol(pl::g_wait_limit_ns, &ns, sizeof(ns));
+}
+
+}  // namespace pl_module
+
 namespace {
 
 #define PL_CUDA(call)                                                     \
@@ -73,14 +81,26 @@ int sm_count() {
 constexpr int kMaxBlocks = 160;
 
 // Shared memory above 48 KB is an attribute of a kernel on each device: set
-// the first time this kernel launches there.
+// the first time this kernel launches there.  With regs, the kernel's
+// warpgroups share out exactly that many registers a thread (setmaxnreg): from
+// a smaller allocation an increase would wait for good, so another count is
+// refused.
 template <typename K>
-int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done) {
+int allow_smem(K kern, int bytes, std::atomic<unsigned long long>& done, int regs = 0) {
   int dev = 0;
   PL_CUDA(cudaGetDevice(&dev));
   const unsigned long long bit = dev < 64 ? 1ull << dev : 0ull;
   if (bit && (done.load(std::memory_order_acquire) & bit)) return PL_OK;
   PL_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (regs) {
+    cudaFuncAttributes at;
+    PL_CUDA(cudaFuncGetAttributes(&at, kern));
+    if (at.numRegs != regs) {
+      std::fprintf(stderr, "pl_attn: a kernel has %d registers a thread instead of %d\n",
+                   at.numRegs, regs);
+      return PL_EFAIL;
+    }
+  }
   done.fetch_or(bit, std::memory_order_release);
   return PL_OK;
 }
@@ -295,7 +315,7 @@ struct Attend {
     ch.part = work_part(c);
     ch.sums = work_sums(c);
     ch.arrived = work_arrived(c);
-    int rc = allow_smem(kern, smem, done);
+    const int rc = allow_smem(kern, smem, done, pl::kChLaunchRegs);
     if (rc) return rc;
     const int blocks = sm_count() < kMaxBlocks ? sm_count() : kMaxBlocks;
     return launch(kern, dim3(blocks), pl::kChThreads, smem, st, true, ch);
@@ -645,14 +665,17 @@ int pl_kv8_read_dev(const pl_kv8* c, int layer, int n, const int* d_seqs, const 
 int pl_kv8_status(const pl_kv8* c, void* stream) {
   const int rc = check_kv8(c);
   if (rc) return rc;
-  PL_CUDA(cudaStreamSynchronize(static_cast<cudaStream_t>(stream)));
+  // all in the stream's order: a stream that does not wait for the default
+  // one could otherwise see the clearing after its next call
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint32_t w = 0;
   uint32_t* err = &static_cast<pl::Kv8Head*>(c->work)->err;
-  PL_CUDA(cudaMemcpy(&w, err, sizeof(w), cudaMemcpyDeviceToHost));
-  if (w) PL_CUDA(cudaMemset(err, 0, sizeof(w)));
+  PL_CUDA(cudaMemcpyAsync(&w, err, sizeof(w), cudaMemcpyDeviceToHost, st));
+  PL_CUDA(cudaStreamSynchronize(st));
+  if (w) PL_CUDA(cudaMemsetAsync(err, 0, sizeof(w), st));
   if (w & (pl::ERR_TIMEOUT_FULL | pl::ERR_TIMEOUT_EMPTY | pl::ERR_TIMEOUT_MMA)) {
     // a block that gave up has not counted itself
-    PL_CUDA(cudaMemset(work_arrived(c), 0, arrive_bytes(c)));
+    PL_CUDA(cudaMemsetAsync(work_arrived(c), 0, arrive_bytes(c), st));
     return PL_ETIMEOUT;
   }
   if (w & pl::ERR_BAD_ARG) return PL_EARG;

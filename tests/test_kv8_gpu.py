@@ -574,3 +574,105 @@ def test_captured_step_replayed():
         want, most, vmax = c.reference([0, 1, 2], [1, 1, 1], q)
         assert bool(((out.double() - want).abs() <= attention_bound(pb.PL_F32, 64, 140, most, vmax, want)).all())
     del graph
+
+
+# ---------------------------------------------------------- less usual calls
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("split", [1, 7, 8, 9, 15])
+def test_append_joins_a_block_of_wide_heads(fmt, split):
+    """Two warps share a block of 16 rows of 128 elements: the scale and the
+    kept rows cross between them, whichever of them holds the new rows."""
+    gen = generator(21)
+    c = Cache(4, 2, 128, fmt)
+    k, v = randn(gen, 16, 256), randn(gen, 16, 256)
+    k[split:] *= 40
+    v[15] *= 40
+    c.resize([0], [split])
+    c.append([0], [split], k[:split], v[:split], pb.PL_F32)
+    kr = rotate(k.double().reshape(16, 2, 128), torch.arange(16, device="cuda"), c.freq, c.gain, c.layout)
+    vr = v.double().reshape(16, 2, 128)
+    old = c.values(0, split).clone()
+    page = int(c.table[0, 0])
+    old_s = c.scales[page, 0, :, :, 0].double().clone()
+    for kv, x in ((0, kr), (1, vr)):
+        check_rows(c, 0, 0, split, x[:split], kv)
+    c.resize([0], [16])
+    c.append([0], [16 - split], k[split:], v[split:], pb.PL_F32)
+    s = c.scales[page, 0, :, :, 0].double()
+    assert bool((s > old_s).all())
+    # the new rows to half a step; the kept ones to half a step of the new scale from what they were,
+    # the ratio of the scales, its product and the code's value rounded once each
+    got = c.values(0, 16)
+    for kv, x in ((0, kr), (1, vr)):
+        check_rows(c, 0, split, 16, x[split:], kv)
+        step = s[:, kv][:, None]
+        half = 0.5 * step if fmt == pb.PL_KV8_INT8 else torch.maximum(old[kv].abs() / 16, step * 2.0 ** -10)
+        assert bool(((got[kv, :split] - old[kv]).abs() <= half * (1 + 2.0 ** -15)).all())
+
+
+@pytest.mark.parametrize("row", [0, 7, 8, 15])
+def test_append_of_a_nonfinite_wide_row(row):
+    c = Cache(2, 2, 128)
+    c.resize([0], [16])
+    k, v = torch.zeros(16, 256, device="cuda"), torch.zeros(16, 256, device="cuda")
+    k[row, 5], v[row, 200] = -math.inf, math.nan
+    c.append([0], [16], k, v, pb.PL_F32)
+    got = c.values(0, 16)
+    assert bool(torch.isnan(got[0, :, 0]).all()) and bool((got[0, :, 1] == 0).all())
+    assert bool(torch.isnan(got[1, :, 1]).all()) and bool((got[1, :, 0] == 0).all())
+
+
+def test_attention_may_name_a_slot_twice():
+    gen = generator(22)
+    c = Cache(8, 2, 64, n_pages=64, n_seqs=3, max_pages=8)
+    c.fill([0, 1, 2], [300, 77, 512], gen)
+    for seqs, counts in (([2, 0, 2, 2], [1] * 4), ([0, 0, 1, 0], [40, 40, 3, 7])):
+        attend_and_check(c, seqs, counts, pb.PL_F32, gen)
+
+
+def test_status_on_a_stream_that_waits_for_no_other():
+    """An error after one that was read is not lost to the clearing of it."""
+    c = Cache(4, 2, 64, n_seqs=2)
+    bad, n = i32([5]), i32([3])
+    with torch.cuda.stream(torch.cuda.Stream()):
+        torch.cuda.current_stream().wait_stream(torch.cuda.default_stream())
+        for _ in range(50):
+            c.c.resize_dev(1, bad.data_ptr(), n.data_ptr(), stream())
+            assert c.c.status(stream()) == pb.PL_EARG
+        assert c.c.status(stream()) == pb.PL_OK
+    torch.cuda.synchronize()
+
+
+def test_two_caches_on_two_streams():
+    """Caches are independent: their calls may overlap."""
+    gen = generator(23)
+    caches = [Cache(8, 2, hd, n_pages=130, n_seqs=2, max_pages=64) for hd in (64, 128)]
+    runs = []
+    for c in caches:
+        c.fill([0, 1], [3000, 4000], gen)
+        q = randn(gen, 130, 8 * c.head_dim)
+        runs.append((c, q, [torch.empty_like(q) for _ in range(2)], i32([0, 1]), i32([0, 65, 130]), torch.cuda.Stream()))
+    for alone in (True, False):
+        torch.cuda.synchronize()
+        for _ in range(1 if alone else 8):
+            for c, q, out, s, st, on in runs:
+                c.c.attend_dev(0, 2, s.data_ptr(), st.data_ptr(), 130, 65, pb.PL_F32, q.data_ptr(), q.stride(0),
+                               out[alone].data_ptr(), q.stride(0), on.cuda_stream)
+                if alone:
+                    torch.cuda.synchronize()
+    for c, _, out, _, _, on in runs:
+        assert c.c.status(on.cuda_stream) == pb.PL_OK
+        assert torch.equal(out[0], out[1])
+
+
+def test_many_entries_of_one_call():
+    """As many entries as a call takes, most of them short and some empty."""
+    gen = generator(24)
+    n = 1024
+    c = Cache(2, 1, 64, n_pages=1500, n_seqs=n, max_pages=2)
+    lens = [(7 * i) % 97 for i in range(n)]
+    c.fill(list(range(n)), lens, gen)
+    attend_and_check(c, list(range(n)), [1] * n, pb.PL_BF16, gen)
+    attend_and_check(c, list(range(n)), [min(m, (3 * i) % 5) for i, m in enumerate(lens)], pb.PL_BF16, gen)
+    c.resize(list(range(n)))
+    assert int(c.refs.abs().sum()) == 0
