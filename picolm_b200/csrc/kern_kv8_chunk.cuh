@@ -9,7 +9,7 @@
 // entry and KV head: row r of a slot is token r / G, query head r % G of the
 // G heads that share the KV head, so a few tokens already fill a tile and
 // both slots read the same K/V tiles.  The K/V tiles of all items, in order,
-// form one list in which every item starts with kChItemCost empty places
+// form one list in which every item starts with kItemCost empty places
 // (what its start and end cost, in tiles), and every block (one per SM)
 // takes an equal contiguous slice of it: long prompts balance by themselves,
 // and few tokens over a long context are split along it.  The part of an
@@ -65,8 +65,6 @@ static_assert(256 * kChSoftmaxRegs + 128 * kChConvertRegs + 128 * kChOtherRegs <
                   kChThreads * kChLaunchRegs,
               "register split exceeds the launch allocation");
 constexpr int kChQueue = 4;            // segments between the scheduler and the others
-constexpr int kChItemCost = 3;         // places of the list before an item's tiles
-constexpr int kChMinPlaces = 6;        // of a block's slice, at least
 constexpr float kChBase = 16.f;        // weight of a row's maximum under the largest scale
 constexpr float kChRescaleLog2 = 8.f;  // raise the running maximum only past 2^8
 constexpr float kChRefGrowth = 4.f;    // raise the scale reference only past 4x
@@ -101,6 +99,14 @@ struct ChShape {
   }
   static_assert(2 * kBN + 2 * HD + 2 * kPCols + (kSumsInTmem && PARTS == 2 ? 2 * HD : 0) <= 512,
                 "TMEM columns");
+  // Places of the list before an item's tiles: what its start (rows of q) and
+  // end (O, a merge) take, in tiles; more where the rows are longer.  1 x 2048
+  // tokens / 4 x 1024 behind 8192 rows / 16 x 64 behind 1024, in us, at
+  // head_dim 64 in FP32: 106, 518, 59 with 3; 98, 502, 55 with 7; 104, 502,
+  // 53 with 12.  At head_dim 128 in BF16: 121, 477, 70 with 3; 107, 465, 61
+  // with 7; 104, 461, 61 with 9; 107, 461, 61 with 12.
+  static constexpr int kItemCost = HD == 64 ? 7 : 9;
+  static constexpr int kMinPlaces = kItemCost + 1;  // of a block's slice, at least
   static constexpr int kPartFloats = 2 * kChRows * (HD + 2);  // a partial: [slot][o.., m, l][row]
 };
 
@@ -237,7 +243,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
     long long places = 0;
     if (ok)
       for (int f = lane * per_item; f < en.n_tok; f += 32 * per_item)
-        places += kChItemCost + ch_tiles<BN>(en.len, en.n_tok, f, per_item);
+        places += Sh::kItemCost + ch_tiles<BN>(en.len, en.n_tok, f, per_item);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) places += __shfl_xor_sync(0xffffffffu, places, d);
     if (lane == 0) sm.prefix[i] = places * heads;
@@ -286,7 +292,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       // --------------------------------------------------------- scheduler
       if (lane == 0) {
         const long long total = sm.prefix[a.n];
-        const long long most = (total + kChMinPlaces - 1) / kChMinPlaces;
+        const long long most = (total + Sh::kMinPlaces - 1) / Sh::kMinPlaces;
         const long long blocks = most < gridDim.x ? most : gridDim.x;
         const int blk = blockIdx.x;
         auto block_of = [&](long long p) {
@@ -308,13 +314,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           int h = static_cast<int>((p - at) / per_head), first = 0;
           at += h * per_head;
           int tiles = ch_tiles<BN>(en.len, en.n_tok, 0, per_item);
-          while (p >= at + kChItemCost + tiles) {
-            at += kChItemCost + tiles;
+          while (p >= at + Sh::kItemCost + tiles) {
+            at += Sh::kItemCost + tiles;
             first += per_item;
             tiles = ch_tiles<BN>(en.len, en.n_tok, first, per_item);
           }
           while (true) {
-            const long long t0 = at + kChItemCost;  // place of the item's first tile
+            const long long t0 = at + Sh::kItemCost;  // place of the item's first tile
             ChSeg g;
             g.j0 = p > t0 ? static_cast<int>(p - t0) : 0;
             g.j1 = end - t0 < tiles ? static_cast<int>(end - t0) : tiles;
