@@ -2,8 +2,8 @@
 // 8-bit paged cache, on the 5th-generation tensor cores (tcgen05 + TMEM).
 //
 // Bound by the softmax (its exponentials and the work around them) and, for
-// FP32 activations, by the tensor pipe, which then runs every product twice
-// (high part and residual).
+// FP32 and FP16 activations, by the tensor pipe, which then runs every product
+// twice (high part and residual).
 //
 // Work.  A query item is up to two 128-row tiles ("slots" A and B) of one
 // entry and KV head: row r of a slot is token r / G, query head r % G of the
@@ -40,16 +40,19 @@
 // maximum; V's goes into the weight, relative to a reference that is raised
 // (with O rescaled) when a scale outgrows it fourfold, as the running
 // maximum is when a score outgrows it by 2^8, so weights stay below 2^14.
-// q is scaled by a power of two a row.  FP32 activations (PARTS 2): q and
+// q is scaled by a power of two a row.  FP32 and FP16 activations (PARTS 2): q and
 // the weights are FP16 high part + residual, and every few tiles O is added
 // to sums with one rounded FP32 operation and starts from zero again: the
 // tensor core truncates as it accumulates, which alone put the output off by
 // 1.6e-8 for each 16 rows, always towards zero.
-// Sixteen-bit ones (PARTS 1): q and the weights are rounded to FP16 once,
-// 2^-12 relative, half or less of what rounding the output to its type costs.
+// BF16 ones (PARTS 1): q and the weights are rounded to FP16 once, at most
+// 2^-11 relative, an eighth of what rounding the output to BF16 costs.  FP16
+// ones too would be off by 1.7 times the rounding of their output.
 #pragma once
 #include <cstdint>
 #include <cuda.h>
+
+#include <type_traits>
 
 #include "kern_kv8_attn.cuh"
 
@@ -68,6 +71,12 @@ constexpr int kChQueue = 4;            // segments between the scheduler and the
 constexpr float kChBase = 16.f;        // weight of a row's maximum under the largest scale
 constexpr float kChRescaleLog2 = 8.f;  // raise the running maximum only past 2^8
 constexpr float kChRefGrowth = 4.f;    // raise the scale reference only past 4x
+
+// FP16 parts of q and of the weights.
+template <typename T>
+constexpr int ch_parts() {
+  return std::is_same<T, __nv_bfloat16>::value ? 1 : 2;
+}
 
 template <int HD, int PARTS>
 struct ChShape {
@@ -171,7 +180,7 @@ __device__ __forceinline__ float2 turn(float2 a, float2 b) {
 template <typename T, int HD, int FMT>
 __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
     const __grid_constant__ Kv8ChunkArgs ca) {
-  constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+  constexpr int PARTS = ch_parts<T>();
   using Sh = ChShape<HD, PARTS>;
   constexpr int BN = Sh::kBN, KS = Sh::kKStages, VS = Sh::kVStages, RS = Sh::kRaw;
   extern __shared__ uint8_t smem_raw[];

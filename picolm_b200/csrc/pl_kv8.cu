@@ -305,7 +305,7 @@ struct Attend {
       d.a = a;
       return run_decode<T, HD, FMT, false>(c, d, st);
     }
-    constexpr int PARTS = sizeof(T) == 4 ? 2 : 1;
+    constexpr int PARTS = pl::ch_parts<T>();
     constexpr int smem = static_cast<int>(sizeof(pl::ChSmem<HD, PARTS>)) + 1024;
     static_assert(smem <= 227 * 1024, "shared memory of the chunk attention");
     static std::atomic<unsigned long long> done{0};

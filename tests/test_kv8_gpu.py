@@ -665,6 +665,21 @@ def test_two_caches_on_two_streams():
         assert torch.equal(out[0], out[1])
 
 
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("counts", [[1, 1], [200, 3]])
+def test_fp16_is_off_by_its_output_alone(head_dim, counts):
+    """FP16 activations are carried as FP32 ones are, and the output is
+    rounded once: half a step of 2^-11, or half a subnormal's 2^-25."""
+    gen = generator(25)
+    c = Cache(8, 2, head_dim, n_pages=40, n_seqs=2, max_pages=20)
+    c.fill([0, 1], [700, 1200], gen)
+    q = randn(gen, sum(counts), 8 * head_dim, dtype=torch.float16)
+    out = c.attend([0, 1], counts, q, torch.empty_like(q), pb.PL_F16)
+    want, most, vmax = c.reference([0, 1], counts, q)
+    bound = attention_bound(pb.PL_F32, head_dim, 1200, most, vmax, want) + want.abs() * 2.0 ** -11 + 2.0 ** -25
+    assert bool(((out.double() - want).abs() <= bound).all())
+
+
 def test_many_entries_of_one_call():
     """As many entries as a call takes, most of them short and some empty."""
     gen = generator(24)
