@@ -454,7 +454,9 @@ int  pl_rope_rows_dev(const pl_rope *r, int dtype, int n, const int *d_pos,
  *
  * One stream at a time per cache: its calls share the workspace, so calls
  * that could overlap on the GPU (two streams, two captured graphs) must be
- * ordered by the caller.  Different caches are independent.  The current
+ * ordered by the caller.  Different caches are independent.  A kernel starts
+ * while the one queued before it on `stream` finishes (programmatic dependent
+ * launch) and reads arrays only after that.  The current
  * device must be the cache's (PL_EDEVICE).  Arrays of a call are device
  * memory; a slot, row count or page out of range that a kernel finds there
  * leaves its entry (its call, for the page operations) undone, or the entry's

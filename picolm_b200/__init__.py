@@ -10,6 +10,9 @@ no usable sm_100 device, calls raise :class:`PlAttnError`.
 ``Attn`` mirrors the C entry points one for one and keeps their argument
 meaning; host-buffer methods take numpy arrays, ``*_dev`` methods take raw
 device pointers (ints), e.g. ``torch.Tensor.data_ptr()``.
+
+``Rope`` (rotary positions as an operator of their own) and ``Kv8Cache`` (the
+8-bit paged KV cache) need no ``Attn``: every call takes what it works on.
 """
 from __future__ import annotations
 

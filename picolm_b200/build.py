@@ -4,9 +4,9 @@
 
 nvcc compiles csrc/pl_attn.cu (the FP16 cache and everything around it) and
 csrc/pl_kv8.cu (rotary positions and the 8-bit paged cache), which include
-the kernel headers, for sm_100a only and links the CUDA runtime statically.  The driver API entry
-point the module needs (cuTensorMapEncodeTiled) is looked up at run time
-through cudaGetDriverEntryPoint, so the library has no link-time dependency
+the kernel headers, for sm_100a only and links the CUDA runtime statically.
+The driver API entry point the module needs (cuTensorMapEncodeTiled) is looked
+up at run time through cudaGetDriverEntryPoint, so the library has no link-time dependency
 on libcuda and loads on a host without a GPU (its calls then fail with
 PL_EDEVICE).  ptxas' resource report (registers, spills per kernel) is
 kept beside the library in libpl_attn.resources.json, and the build fails if

@@ -58,6 +58,15 @@ constexpr int kKv8MaxGroup = 8;  // query heads per KV head
 // one rounded FP32 FMA: the tensor core truncates as it accumulates, and
 // over a long segment that would add up in one direction.
 //
+// On one B200: 64 sequences of 2048 rows, 32/4 heads of 64, FP32: 26 us (69
+// MB); 32 ragged ones up to 8192 rows, 32/8 heads of 128, BF16: 85 us (335
+// MB, 3.9 TB/s); one of 32768, 32/8 of 64: 20 us; one of 256 rows: 10 us.  Of
+// the 26 us about 11 stream the tiles, at 5.9 TB/s; before that a block reads
+// and scans the books (1.3), finds its first tile (2.5) and rotates q (0.8),
+// and after it the runs that cross blocks are merged (5).  At head_dim 128
+// the stream runs at the pace of its eight warps, which have 255 registers
+// each; more warps spill and are slower, as were four of 64-row tiles.
+//
 // Segments of a run in several warps of a block are merged in shared
 // memory by the warp where the run starts; runs over several blocks leave
 // one partial a block in the workspace, and the block that finishes a run's

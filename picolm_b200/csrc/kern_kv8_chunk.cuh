@@ -36,6 +36,13 @@
 // a tile is kept short: unrolled over 128 columns, two slots at different
 // places of it waited for instructions four cycles in five.
 //
+// Measured on one B200: a prompt of 2048 FP32 tokens, 32/4 heads of 64: 92 us
+// (17 GFLOP, 187 TFLOP/s; the tensor pipe, which does it twice, is active
+// 18% of the time, issue slots 45%); 4 chunks of up to 1024 BF16 tokens
+// behind up to 8192 rows, 32/8 heads of 128: 461 us (682 TFLOP/s, 32%, 50%).
+// A pair of tiles takes 1.5 to 1.8 us, of which 2^x alone would take 0.55;
+// the start and the end of an item another 7 to 9 pairs' time.
+//
 // Scales and ranges.  K's scale multiplies 16 columns of S before the row
 // maximum; V's goes into the weight, relative to a reference that is raised
 // (with O rescaled) when a scale outgrows it fourfold, as the running

@@ -9,10 +9,15 @@
 // respect to x) is the same with -s.  There is no table of positions: the
 // angle is taken in FP64, so a position may be any non-negative int.
 //
-// Bound by HBM: each element is read and written once (8192 rows of 32 + 8
-// heads of 128 in BF16: 168 MB).  A block rotates all heads of a few rows,
-// so that the FP64 cosines (about a hundred instructions each) are computed
-// once per (row, pair) into shared memory and not once per head.
+// Bound by HBM: each element is read and written once.  A block rotates all
+// heads of a few rows, so that the FP64 cosines (about a hundred instructions
+// each) are computed once per (row, pair) into shared memory and not once
+// per head.  8192 rows of 32 + 8 heads of 128 in BF16, half of each rotated
+// (168 MB), on one B200: 46 us, 3.7 TB/s, 57% of a copy; the rest is a block's
+// start, whose cosines and first rows nothing else of the block overlaps.
+// On the way: an element a thread 125 us; runs of 16 bytes 78; a thread's
+// place found once for all rows 53; blocks of equal width, two rows under
+// way instead of four for more blocks an SM 46.  64 FP32 rows: 10 us.
 #pragma once
 #include <cstdint>
 #include <cuda_bf16.h>
@@ -198,7 +203,8 @@ __global__ void __launch_bounds__(kRopeThreads) rope_rows_any_kernel(
 // Aligned rows.  A unit is eight elements of a head (LLaMA; past dim: copied)
 // or the two runs of eight that rotate together (Qwen, dim / 2 a multiple of
 // eight).  A thread keeps its unit over the block's rows, so its place is
-// found once, and has the loads of four rows under way.
+// found once, and has the loads of four (Qwen: two, of two runs) rows under
+// way.
 template <typename T, bool LLAMA>
 __global__ void __launch_bounds__(kRopeThreads, sizeof(T) == 4 ? 2 : 3) rope_rows_kernel(
     const __grid_constant__ RopeRowsArgs a) {

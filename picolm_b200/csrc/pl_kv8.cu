@@ -160,7 +160,8 @@ int check_kv8_shape(const pl_kv8* c) {
   if (static_cast<double>(c->n_pages) * c->n_layers * c->n_kv_heads * 2 > 2147483647.0)
     return PL_EUNSUPPORTED;
   if (c->rope.dim < 0 || (c->rope.dim & 1) || c->rope.dim > c->head_dim ||
-      (c->rope.dim && c->rope.head_dim != c->head_dim))
+      (c->rope.dim && (c->rope.head_dim != c->head_dim ||
+                       (c->rope.type != PL_ROPE_LLAMA && c->rope.type != PL_ROPE_QWEN))))
     return PL_EARG;
   return PL_OK;
 }
@@ -427,7 +428,8 @@ int pl_rope_rows_dev(const pl_rope* r, int dtype, int n, const int* d_pos, int n
   if (!r || !good_dtype(dtype) || n < 0 || n_heads < 0 || n_kv_heads < 0 ||
       n_heads > 65536 || n_kv_heads > 65536 || r->head_dim < 8 ||
       r->head_dim > 2 * PL_ROPE_MAX_PAIRS || r->head_dim % 8 || r->dim < 0 ||
-      r->dim > r->head_dim || (r->dim & 1))
+      r->dim > r->head_dim || (r->dim & 1) ||
+      (r->type != PL_ROPE_LLAMA && r->type != PL_ROPE_QWEN))
     return PL_EARG;
   if (n == 0 || n_heads + n_kv_heads == 0) return PL_OK;
   const size_t es = elem_size(dtype);

@@ -115,3 +115,13 @@ def test_struct_sizes_match_the_header(tmp_path):
     subprocess.run(["gcc", "-std=c11", "-I", os.path.dirname(pb.HEADER), "-o", str(tmp_path / "size"), str(src)], check=True)
     got = subprocess.run([str(tmp_path / "size")], check=True, capture_output=True, text=True).stdout.split()
     assert [int(x) for x in got] == [C.sizeof(pb._RopeStruct), C.sizeof(pb._Kv8Struct), pb._Kv8Struct.codes.offset]
+
+
+def test_layouts_that_do_not_exist_are_refused():
+    r = pb.Rope(64)
+    r.struct.type = 2
+    P = 4096
+    assert pb.load().pl_rope_rows_dev(r._p, 0, 1, P, 2, P, 128, P, 128, 0, None, 0, None, 0, 0, None) == pb.PL_EARG
+    c = pb.Kv8Cache(**GOOD, rope=r, codes=256, scales=256, table=256, lens=256, refs=256, work=256,
+                    work_bytes=pb.kv8_work_bytes(**GOOD))
+    assert pb.load().pl_kv8_status(c._p, None) == pb.PL_EARG

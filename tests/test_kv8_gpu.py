@@ -691,3 +691,18 @@ def test_many_entries_of_one_call():
     attend_and_check(c, list(range(n)), [min(m, (3 * i) % 5) for i, m in enumerate(lens)], pb.PL_BF16, gen)
     c.resize(list(range(n)))
     assert int(c.refs.abs().sum()) == 0
+
+
+def test_the_integration_guide_runs():
+    """The Python example of the guide, as written."""
+    import pathlib
+    import re
+
+    text = (pathlib.Path(__file__).resolve().parent.parent / "INTEGRATION.md").read_text()
+    blocks = [b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "Kv8Cache" in b]
+    assert len(blocks) == 1
+    scope = {}
+    exec(blocks[0], scope)
+    # one row attends itself: the output is v, a head for each group of 8, to int8
+    want = scope["v"].view(2, 4, 1, 64).expand(2, 4, 8, 64).reshape(2, 2048)
+    assert float((scope["out"] - want).abs().max()) <= float(want.abs().max()) / 127 * 0.51
