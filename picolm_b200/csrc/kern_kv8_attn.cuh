@@ -490,7 +490,7 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
   auto place_tile = [&](int page) {
     if (page < 0 || page >= a.g.n_pages) {
       atomicOr(&a.g.head->err, ERR_BAD_ARG);
-      page = 0;
+      page = 0;  // read instead; a row is not appended there
     }
     t_slab = static_cast<int>(a.g.slab(page, t_run % heads, 0));
   };
@@ -579,7 +579,9 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
     constexpr int E = HD / 32;
     float kx[E], vx[E];
     const bool appends = APPEND && seen <= TR;
+    int page = -1;
     if (appends) {
+      page = a.g.table[static_cast<long long>(sm.slot[i]) * a.g.max_pages + row0 / kPage];
       for (int p = lane; p < a.rope.dim >> 1; p += 32)
         sm.cs[warp][p] = rope_cs(sm.half_turns[p], a.rope.gain, len - 1);
       const T* k = static_cast<const T*>(da.k) + i * da.k_stride + h * HD;
@@ -607,7 +609,7 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
       ok = false;
       break;
     }
-    if (appends) {
+    if (appends && page >= 0 && page < a.g.n_pages) {
       const int r = seen - 1, block = r / kBlock * kBlock;
       const long long slab = __shfl_sync(0xffffffffu, c_slab, x - c_base);
       const int b = (row0 % kPage + block) / kBlock;

@@ -665,6 +665,27 @@ def test_two_caches_on_two_streams():
         assert torch.equal(out[0], out[1])
 
 
+@pytest.mark.parametrize("page", [-1, 1000])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_decode_without_a_page_writes_nothing(page, head_dim):
+    """A new row whose page is missing is not written anywhere; another entry's step is made."""
+    gen = generator(26)
+    c = Cache(4, 2, head_dim, n_seqs=3)
+    c.fill([0, 1, 2], [40, 129, 64], gen)
+    at = int(c.table[2, 0])
+    c.table[1, 2] = page
+    codes, scales = c.codes.clone(), c.scales.clone()
+    q, k, v = randn(gen, 2, 4 * head_dim), randn(gen, 2, 2 * head_dim), randn(gen, 2, 2 * head_dim)
+    out, s = torch.empty_like(q), i32([1, 2])
+    c.c.decode_dev(0, 2, s.data_ptr(), pb.PL_F32, q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0),
+                   v.data_ptr(), v.stride(0), out.data_ptr(), out.stride(0), stream())
+    assert c.c.status(stream()) == pb.PL_EARG
+    changed = (c.codes != codes).flatten(1).any(1) | (c.scales.nan_to_num(9) != scales.nan_to_num(9)).flatten(1).any(1)
+    assert changed.nonzero().flatten().tolist() == [at]
+    want, most, vmax = c.reference([2], [1], q[1:])
+    assert bool(((out[1:].double() - want).abs() <= attention_bound(pb.PL_F32, head_dim, 64, most, vmax, want)).all())
+
+
 @pytest.mark.parametrize("head_dim", [64, 128])
 @pytest.mark.parametrize("counts", [[1, 1], [200, 3]])
 def test_fp16_is_off_by_its_output_alone(head_dim, counts):
