@@ -44,9 +44,10 @@
 // the start and the end of an item another 7 to 9 pairs' time.
 //
 // Scales and ranges.  K's scale multiplies 16 columns of S before the row
-// maximum; V's goes into the weight, relative to a reference that is raised
-// (with O rescaled) when a scale outgrows it fourfold, as the running
-// maximum is when a score outgrows it by 2^8, so weights stay below 2^14.
+// maximum; V's goes into the weight, relative to a reference of the row (of
+// the blocks that it sees) that is raised (with O rescaled) when a scale
+// outgrows it fourfold, as the running maximum is when a score outgrows it by
+// 2^8, so weights stay below 2^14.
 // q is scaled by a power of two a row.  FP32 and FP16 activations (PARTS 2): q and
 // the weights are FP16 high part + residual, and every few tiles O is added
 // to sums with one rounded FP32 operation and starts from zero again: the
@@ -794,6 +795,13 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
             if (c > lim) u[c] = __float_as_uint(-INFINITY);
             asm volatile("" : "+r"(u[c]));  // a branch, not 64 selects in every tile
           }
+          // blocks that are hidden whole weigh nothing and leave the row's
+          // reference where it is: later tokens' values do not reach this one
+#pragma unroll
+          for (int b = 0; b < Sh::kBlocks; ++b) {
+            if (16 * b > lim) sv[b] = 0.f;
+            asm volatile("" : "+f"(sv[b]));
+          }
         }
         // ---- the row's maximum: of a block's columns, times its scale (which
         // is not negative), over the blocks
@@ -808,8 +816,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           m_tile = fmaxf(m_tile, z * sk[b]);
         }
         const float top_v = max3(fmaxf(sv[0], sv[1]), sv[2], sv[3]);
-        const bool rescale = __any_sync(0xffffffffu, m_tile > m_used + kChRescaleLog2) ||
-                             top_v > kChRefGrowth * ref;
+        const bool rescale = __any_sync(
+            0xffffffffu, m_tile > m_used + kChRescaleLog2 || top_v > kChRefGrowth * ref);
         const bool moved = PARTS == 2 && j > 0 && j % Sh::kFlushTiles == 0;
         // O and P are free to change once PV of the tile before is done
         if (A >= 1 && !mbar_wait_short(&sm.pv_done[x][(A - 1) & 1], ((A - 1) >> 1) & 1))

@@ -205,6 +205,39 @@ def test_large_and_small_magnitudes(count):
         attend_and_check(c, [0], [count], pb.PL_F32, gen, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("length", [100, 320])
+def test_later_values_do_not_reach_earlier_tokens(fmt, head_dim, length):
+    """A prompt whose V scales rise from block to block: the masked blocks of
+    a tile are up to 10^13 times larger than the ones that a token sees.
+
+    attention_bound holds with each token's own largest |v|, the largest
+    scale of the blocks that it sees times the largest code: a weight in two
+    FP16 parts is off by 2^-25 at least, in units of which the largest visible
+    scale is 16 to 64, so by no more than `rows` 2^-29 of that |v| over all
+    rows, which the bound's 2 rows 2^-24 covers."""
+    gen = generator(31)
+    c = Cache(8, 2, head_dim, fmt, n_pages=32, n_seqs=1, max_pages=16)
+    c.fill([0], [length], gen)
+    pages = c.table[0, :-(-length // PAGE)].long()
+    for dtype, lo, hi in ((pb.PL_F32, -20, 12), (pb.PL_BF16, -20, 12), (pb.PL_F16, -5, 2)):
+        saved = c.scales.clone()
+        rise = torch.linspace(lo, hi, 4 * len(pages), device="cuda").view(-1, 1, 4)
+        c.scales[pages, 0, :, 1] *= 10.0 ** rise
+        q = randn(gen, length, 8 * head_dim, dtype=TORCH[dtype])
+        out = c.attend([0], [length], q, torch.empty_like(q), dtype)
+        want, most, _ = c.reference([0], [length], q)
+        top = c.scales[pages, 0, :, 1].permute(1, 0, 2).reshape(2, -1).double()  # [kv head][block]
+        top = torch.nan_to_num(top, 0.0).cummax(1).values * TOP[fmt]
+        vmax = top.repeat_interleave(BLOCK, 1)[:, :length].t()                   # [token][kv head]
+        vmax = vmax.repeat_interleave(4 * head_dim, 1)
+        err = (out.double() - want).abs()
+        assert bool((err <= attention_bound(dtype, head_dim, length, most, vmax, want)).all()), float(
+            (err / vmax).max())
+        c.scales.copy_(saved)
+
+
 def test_nan_stays_where_it_is():
     """A NaN block is seen by tokens that attend it, by no others; a NaN in q
     by its own head and token."""
