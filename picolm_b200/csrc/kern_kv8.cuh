@@ -194,7 +194,9 @@ __device__ __forceinline__ float quotient(float x, float by, float inv) {
 // code; rows that the block held before are kept, rescaled when the new
 // rows raise the scale (code' = round(code * old / new)).  A row with a
 // NaN or infinity makes the scale NaN: the whole block then reads as NaN
-// rather than as finite numbers that were never written.
+// rather than as finite numbers that were never written.  Its new codes are 0:
+// e4m3 has a code for NaN, and attention multiplies the codes of rows that a
+// mask hides by a weight of 0, which a NaN would survive.
 //
 // Cosines are FP64 and rounded once, so that codes do not depend on how a
 // row was appended; a block of rows takes two sincospi a pair (its first
@@ -329,6 +331,12 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv8_append_kernel(
     const bool grown = lo > 0 && __float_as_uint(s) != old_bits;
     __syncwarp();  // every lane has read the old scale
     if (lane == 0 && row_first == 0) *sc = s;
+    if (!(s < INFINITY)) {  // no code stands for a NaN: the scale alone says it
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[p][j] = 0.f;
+    }
     if (by > 1e-25f && by < 1e25f) {
 #pragma unroll
       for (int p = 0; p < kPasses; ++p)

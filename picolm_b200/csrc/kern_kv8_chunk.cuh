@@ -563,7 +563,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         }
         if (!is_v && pt < 32) {
           // A scale that is not finite becomes 0 and leaves a bit: rows that see
-          // its block are made NaN, and 0 times what a mask hides stays 0.
+          // its block are made NaN, and 0 times what a mask hides stays 0 (the
+          // codes of rows that exist are never NaN).
           const int kv = pt / Sh::kBlocks & 1, b = pt % Sh::kBlocks;
           const float f = b * kBlock < left ? sm.raw_scale[rs][kv][b] : 0.f;
           const uint32_t odd =

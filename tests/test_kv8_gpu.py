@@ -265,6 +265,45 @@ def test_nan_stays_where_it_is():
     assert torch.isnan(out).any(-1).tolist() == [[True, True, False, False], [False] * 4]
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("one", [False, True], ids=["append", "decode"])
+def test_appended_nonfinite_values_reach_no_earlier_token(fmt, head_dim, value, one):
+    """Rows 80..95 share a scale; row 85 of V (head 0) or of K (head 1) is
+    not finite, appended with the others or by a decode step.  Tokens from
+    row 80 on are NaN in that head; the others are as over a cache that had
+    0 there."""
+    gen = generator(32)
+    kd, n = 2 * head_dim, 86 if one else 100
+    k, v, q = (randn(gen, n, w) for w in (kd, kd, 2 * kd))
+    k[85, head_dim + 3] = v[85, 5] = 0
+    caches = []
+    for bad in (value, 0.0):
+        c = Cache(4, 2, head_dim, fmt, n_seqs=1)
+        k[85, head_dim + 3] = v[85, 5] = bad
+        first = 85 if one else 100
+        c.resize([0], [first])
+        c.append([0], [first], k[:first], v[:first], pb.PL_F32)
+        if one:
+            c.resize([0], [86])
+            out = c.decode([0], q[85:], k[85:], v[85:], torch.empty_like(q[85:]), pb.PL_F32)
+            assert bool(torch.isnan(out).all()) == (bad != 0) and bool(torch.isnan(out).any()) == (bad != 0)
+        caches.append(c)
+    assert bool((caches[0].values(0, n).isnan() == torch.isnan(caches[0].scales[caches[0].table[0, :2].long(), 0])
+                 .repeat_interleave(BLOCK, -1).permute(2, 0, 3, 1).reshape(2, -1, 2, 1)[:, :n]).all())
+    if fmt == pb.PL_KV8_E4M3:  # no NaN among the codes of rows that exist
+        code = caches[0].codes[caches[0].table[0, :2].long(), 0].permute(2, 0, 3, 1, 4).reshape(2, -1, kd)[:, :n]
+        assert bool(((code & 127) != 127).all())
+    for dtype in DTYPES:
+        x = q.to(TORCH[dtype])
+        out = caches[0].attend([0], [n], x, torch.empty_like(x), dtype)
+        want, most, vmax = caches[1].reference([0], [n], x)
+        assert bool(torch.isnan(out[80:]).all()) and not bool(torch.isnan(out[:80]).any())
+        bound = attention_bound(dtype, head_dim, 128, most, vmax, want)
+        assert bool(((out.double() - want).abs() <= bound)[:80].all())
+
+
 @pytest.mark.parametrize("seqs,length", [(1, 20000), (3, 9001)])
 def test_long_contexts_are_split(seqs, length):
     gen = generator(10)
