@@ -446,34 +446,35 @@ struct Kv8PlanArgs {
 };
 
 // Exclusive prefix sum of `v` over the block; the sum of all in `total`.
-__device__ __forceinline__ int block_scan(int v, int& total, int* s_warp) {
+template <typename N>
+__device__ __forceinline__ N block_scan(N v, N& total, long long* s_warp) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int x = v;
+  N x = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, x, d);
+    const N y = __shfl_up_sync(0xffffffffu, x, d);
     if (lane >= d) x += y;
   }
   __syncthreads();  // s_warp may still be read from an earlier scan
   if (lane == 31) s_warp[warp] = x;
   __syncthreads();
   if (warp == 0) {
-    int w = s_warp[lane];
+    N w = static_cast<N>(s_warp[lane]);
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, d);
+      const N y = __shfl_up_sync(0xffffffffu, w, d);
       if (lane >= d) w += y;
     }
     s_warp[lane] = w;
   }
   __syncthreads();
-  total = s_warp[31];
-  return x - v + (warp ? s_warp[warp - 1] : 0);
+  total = static_cast<N>(s_warp[31]);
+  return x - v + (warp ? static_cast<N>(s_warp[warp - 1]) : 0);
 }
 
 __device__ __forceinline__ int pages_of(int rows) { return (rows + kPage - 1) / kPage; }
 
-__device__ void plan_resize(const Kv8PlanArgs& a, int* s_warp, int (*s_e)[kPlanSeqs]) {
+__device__ void plan_resize(const Kv8PlanArgs& a, long long* s_warp, int (*s_e)[kPlanSeqs]) {
   const Kv8Geo& g = a.g;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int* s_slot = s_e[0];
@@ -515,7 +516,8 @@ __device__ void plan_resize(const Kv8PlanArgs& a, int* s_warp, int (*s_e)[kPlanS
   __syncthreads();
   // an entry that grows within a page it shares takes a copy of it; the
   // last sharer of the call keeps the page if nobody else holds it
-  int need = 0, copy = 0;
+  long long need = 0;  // 1024 entries of up to 2^25 pages
+  int copy = 0;
   if (tid < a.n) {
     const int tail = s_tail[tid];
     if (tail >= 0) {
@@ -525,8 +527,9 @@ __device__ void plan_resize(const Kv8PlanArgs& a, int* s_warp, int (*s_e)[kPlanS
     }
     need = max(0, pages_of(s_new[tid]) - pages_of(s_old[tid])) + copy;
   }
-  int total, n_copies;
-  const int off = block_scan(need, total, s_warp);
+  long long wanted;
+  int n_copies;
+  const long long off_wide = block_scan(need, wanted, s_warp);
   const int copy_at = block_scan(copy, n_copies, s_warp);
   // the lowest free pages, in order (each thread a contiguous run of pages)
   const int per = (g.n_pages + kPlanThreads - 1) / kPlanThreads;
@@ -535,7 +538,7 @@ __device__ void plan_resize(const Kv8PlanArgs& a, int* s_warp, int (*s_e)[kPlanS
   for (int p = p0; p < p1; ++p) free_here += __ldcg(&g.refs[p]) == 0;
   int n_free;
   int at = block_scan(free_here, n_free, s_warp);
-  if (total > n_free) {  // nothing is changed: the released pages are taken back
+  if (wanted > n_free) {  // nothing is changed: the released pages are taken back
     for (int i = warp; i < a.n; i += kPlanThreads / 32) {
       const int* row = g.table + static_cast<long long>(s_slot[i]) * g.max_pages;
       for (int j = pages_of(s_new[i]) + lane; j < pages_of(s_old[i]); j += 32) {
@@ -546,6 +549,8 @@ __device__ void plan_resize(const Kv8PlanArgs& a, int* s_warp, int (*s_e)[kPlanS
     if (tid == 0) atomicOr(&g.head->err, ERR_NO_PAGES);
     return;
   }
+  // from here on no more than the pool's pages, fewer than 2^30
+  const int total = static_cast<int>(wanted), off = static_cast<int>(off_wide);
   for (int p = p0; p < p1 && at < total; ++p)
     if (__ldcg(&g.refs[p]) == 0) a.mark[at++] = p;
   if (tid < a.n) s_off[tid] = off | (copy << 31);
@@ -611,7 +616,7 @@ __device__ void plan_fork(const Kv8PlanArgs& a, int (*s_e)[kPlanSeqs]) {
   }
 }
 
-__device__ void plan_compact(const Kv8PlanArgs& a, int* s_warp) {
+__device__ void plan_compact(const Kv8PlanArgs& a, long long* s_warp) {
   const Kv8Geo& g = a.g;
   const int tid = threadIdx.x;
   const int per = (g.n_pages + kPlanThreads - 1) / kPlanThreads;
@@ -671,7 +676,7 @@ __device__ void plan_copy(const Kv8PlanArgs& a) {
 
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(
     const __grid_constant__ Kv8PlanArgs a) {
-  __shared__ int s_warp[32];
+  __shared__ long long s_warp[32];
   __shared__ int s_e[5][kPlanSeqs];
   // the copies may become resident now; they wait for this grid's end
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

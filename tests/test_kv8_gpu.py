@@ -484,6 +484,33 @@ def test_large_pools():
     assert [[p for p in row if p >= 0] for row in c.table.tolist()] == b.pages
 
 
+@pytest.mark.parametrize("n_seqs,max_pages", [(1024, 2 ** 21), (1024, 2 ** 22), (256, 2 ** 23 + 1)])
+def test_more_pages_than_31_bits_count(n_seqs, max_pages):
+    """Entries that want 2^31 pages, 2^32 and 2^31 + 256 between them: too
+    many for the pool, which keeps everything.  (Nothing is written to the
+    table, 8 to 17 GB, so it is left as it was allocated.)"""
+    geometry = dict(n_layers=1, n_heads=1, n_kv_heads=1, head_dim=64, n_pages=300, n_seqs=n_seqs, max_pages=max_pages)
+    codes = torch.zeros(300 * 2 * 64 * 64, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(300 * 8, device="cuda")
+    table = torch.empty(n_seqs * max_pages, dtype=torch.int32, device="cuda")
+    lens, refs = torch.zeros(n_seqs, dtype=torch.int32, device="cuda"), torch.zeros(300, dtype=torch.int32, device="cuda")
+    work = torch.zeros(pb.kv8_work_bytes(**geometry), dtype=torch.uint8, device="cuda")
+    c = pb.Kv8Cache(**geometry, codes=codes.data_ptr(), scales=scales.data_ptr(), table=table.data_ptr(),
+                    lens=lens.data_ptr(), refs=refs.data_ptr(), work=work.data_ptr(), work_bytes=work.numel())
+    seqs, want = i32(list(range(n_seqs))), i32([max_pages * PAGE] * n_seqs)
+    c.resize_dev(n_seqs, seqs.data_ptr(), want.data_ptr(), stream())
+    assert c.status(stream()) == pb.PL_ENOMEM
+    assert not bool(lens.any()) and not bool(refs.any())
+    # and the pool still serves what fits
+    want.fill_(0)
+    want[:300] = 64 if n_seqs >= 300 else 1
+    c.resize_dev(n_seqs, seqs.data_ptr(), want.data_ptr(), stream())
+    assert c.status(stream()) == pb.PL_OK
+    assert torch.equal(lens, want) and int(refs.sum()) == min(n_seqs, 300)
+    del table
+    torch.cuda.empty_cache()
+
+
 # --------------------------------------------------------------- refusals
 def test_bad_entries_are_reported_and_left_undone():
     gen = generator(13)
