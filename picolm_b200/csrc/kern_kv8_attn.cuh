@@ -362,11 +362,10 @@ __device__ __forceinline__ void append_row(const float (&x)[HD / 32], int lane, 
     *s_scale = s;
     *g_scale = s;
   }
-  uint32_t code = 0;  // of the rows of a block without a finite scale, too
-  if (s < INFINITY) {
+  uint32_t code = 0;
 #pragma unroll
-    for (int j = 0; j < E; ++j) code |= encode1<FMT>(__fdiv_rn(x[j], by)) << (8 * j);
-  }
+  for (int j = 0; j < E; ++j) code |= encode1<FMT>(__fdiv_rn(x[j], by)) << (8 * j);
+  if (!(s < INFINITY)) code = 0;  // no code stands for a NaN
   const int el = lane * E;
   const uint32_t at = tile + tile_off<HD>(r, el >> 4) + (el & 15);
   if constexpr (E == 2) {
