@@ -464,7 +464,9 @@ int  pl_rope_rows_dev(const pl_rope *r, int dtype, int n, const int *d_pos,
  * pl_kv8_status as PL_EARG.  Slots of one call are distinct wherever it
  * writes to the cache or its books; attention and read-back may name one
  * several times.  The bound on device-side waits is pl_attn_set_wait_limit's
- * (2 s without a context).  A call has n <= 1024 entries, and fewer than
+ * (2 s without a context); where several tokens attend, one wait may last as
+ * long as a block's share of the rows (about 1 us for 64 of them), and a
+ * call whose waits run out leaves its output undefined.  A call has n <= 1024 entries, and fewer than
  * 2^29 / (max_pages * n_kv_heads) (PL_EARG).
  * Inputs and outputs are `dtype` rows of heads x head_dim elements, 16-byte
  * aligned with strides (in elements) that are multiples of 16 bytes. */

@@ -605,7 +605,7 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
         }
       }
     }
-    if (!mbar_wait_short(&sm.full[warp][s], ((x - x0) / NS) & 1)) {
+    if (!mbar_wait_warp(&sm.full[warp][s], ((x - x0) / NS) & 1)) {
       if (lane == 0) atomicOr(&a.g.head->err, ERR_TIMEOUT_FULL);
       ok = false;
       break;
@@ -749,7 +749,7 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
   }
   // never leave with copies in flight
   for (int x = max(issued - NS, x0); x < issued; ++x)
-    mbar_wait_short(&sm.full[warp][(x - x0) % NS], ((x - x0) / NS) & 1);
+    mbar_wait_drained(&sm.full[warp][(x - x0) % NS], ((x - x0) / NS) & 1);
   __syncthreads();
 
   auto write_run = [&](int r) {

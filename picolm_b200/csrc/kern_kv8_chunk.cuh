@@ -297,10 +297,17 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
   const uint32_t tmem = sm.tmem_base;
 
   // The k-th published segment stays in its place until every role has
-  // released it: a copy of it would cost each thread a dozen registers.
-  auto take = [&](int k) -> bool {
-    return mbar_wait_short(&sm.seg_full[k % kChQueue], (k / kChQueue) & 1) &&
-           sm.seg[k % kChQueue].tiles > 0;
+  // released it: a copy of it would cost each thread a dozen registers.  False
+  // after the last one, and when none came in time, which is recorded.
+  auto taken = [&](int k, bool there) -> bool {
+    if (!there) atomicOr(err, ERR_TIMEOUT_EMPTY);
+    return there && sm.seg[k % kChQueue].tiles > 0;
+  };
+  auto take = [&](int k) -> bool {  // by a whole warp
+    return taken(k, mbar_wait_warp(&sm.seg_full[k % kChQueue], (k / kChQueue) & 1));
+  };
+  auto take_alone = [&](int k) -> bool {  // by one lane of its warp
+    return taken(k, mbar_wait_short(&sm.seg_full[k % kChQueue], (k / kChQueue) & 1));
   };
 
   if (warp >= 12) {
@@ -403,7 +410,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
           }
           const int page = __shfl_sync(0xffffffffu, mine, at - batch);
           const int s = u % RS;
-          if (u >= RS && !mbar_wait_short(&sm.raw_empty[s], ((u / RS) - 1) & 1)) {
+          if (u >= RS && !mbar_wait_warp(&sm.raw_empty[s], ((u / RS) - 1) & 1)) {
             if (lane == 0) atomicOr(err, ERR_TIMEOUT_EMPTY);
             ok = false;
             break;
@@ -427,7 +434,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       }
       // never leave with copies in flight
       for (int w = max(u - RS, 0); w < u; ++w)
-        mbar_wait_short(&sm.raw_full[w % RS], (w / RS) & 1);
+        mbar_wait_drained(&sm.raw_full[w % RS], (w / RS) & 1);
     } else if (lane == 0) {
       // ------------------------------------------------- MMA issuer of slot x
       const int x = warp - 12;
@@ -460,7 +467,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         tc_commit(&sm.v_empty[vs]);
         return true;
       };
-      for (int k = 0; ok && take(k); ++k) {
+      for (int k = 0; ok && take_alone(k); ++k) {
         const ChSeg& g = sm.seg[k % kChQueue];
         const int nt = g.j1 - g.j0;
         const bool active = g.first + x * slot_tok < g.n_tok;
@@ -504,7 +511,7 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       if (!ok) atomicOr(err, ERR_TIMEOUT_MMA);
       // all issued MMAs must finish before TMEM is freed
       tc_commit(&sm.mma_done[x]);
-      mbar_wait_short(&sm.mma_done[x], 0);
+      mbar_wait_drained(&sm.mma_done[x], 0);
     }
   } else if (warp >= 8) {
     regs_dec<kChConvertRegs>();
@@ -523,9 +530,10 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         const bool is_v = w == 2 * nt - 1 || (w > 0 && !(w & 1));
         const int j = is_v ? (w == 2 * nt - 1 ? nt - 1 : w / 2 - 1) : (w + 1) / 2;
         const int n = J + j, rs = u % RS, stages = is_v ? VS : KS, s = n % stages;
-        if (!mbar_wait_short(&sm.raw_full[rs], (u / RS) & 1) ||
-            (n >= stages && !mbar_wait_short(is_v ? &sm.v_empty[s] : &sm.k_empty[s],
-                                               ((n / stages) - 1) & 1))) {
+        if (!__all_sync(0xffffffffu,
+                        mbar_wait_short(&sm.raw_full[rs], (u / RS) & 1) &&
+                            (n < stages || mbar_wait_short(is_v ? &sm.v_empty[s] : &sm.k_empty[s],
+                                                           ((n / stages) - 1) & 1)))) {
           if (lane == 0) atomicOr(err, ERR_TIMEOUT_EMPTY);
           ok = false;
           break;
@@ -757,9 +765,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       for (int j = 0; j < nt && active; ++j, ++A) {
         const int n = J + j;
         // (the scales are the converters' writes: their barriers too)
-        if (ok && !(mbar_wait_short(&sm.scale_full[n & 7], (n >> 3) & 1) &&
-                    mbar_wait_short(&sm.s_full[x], A & 1)))
-          ok = false;
+        ok = __all_sync(0xffffffffu, ok && mbar_wait_short(&sm.scale_full[n & 7], (n >> 3) & 1) &&
+                                         mbar_wait_short(&sm.s_full[x], A & 1));
         if (!ok) continue;
         tc_fence_after();
         uint32_t u[BN];
@@ -820,7 +827,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         const bool rescale = __any_sync(
             0xffffffffu, m_tile > m_used + kChRescaleLog2 || top_v > kChRefGrowth * ref);
         const bool moved = PARTS == 2 && j > 0 && j % Sh::kFlushTiles == 0;
-        // O and P are free to change once PV of the tile before is done
+        // O and P are free to change once PV of the tile before is done (a lane's
+        // verdict joins the others' at the warp's next vote)
         if (A >= 1 && !mbar_wait_short(&sm.pv_done[x][(A - 1) & 1], ((A - 1) >> 1) & 1))
           ok = false;
         tc_fence_after();
@@ -888,7 +896,8 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
                     x * kChRows * (HD + 2) + r;
       if (active) {
         // ---- the segment's O
-        ok = ok && mbar_wait_short(&sm.pv_done[x][(A - 1) & 1], ((A - 1) >> 1) & 1);
+        ok = __all_sync(0xffffffffu,
+                        ok && mbar_wait_short(&sm.pv_done[x][(A - 1) & 1], ((A - 1) >> 1) & 1));
         tc_fence_after();
         if (ok) {
           const float back = ref * (1.f / kChBase);
@@ -937,15 +946,16 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
         __syncwarp();
         if (lane == 0) mbar_arrive(&sm.part_full);
         if (tid == 0) {
-          mbar_wait_short(&sm.part_full, n_merge & 1);
-          const bool done = atomicAdd(&ca.arrived[g.f0], 1) == g.parts - 1;
+          const bool whole_part = mbar_wait_short(&sm.part_full, n_merge & 1);
+          if (!whole_part) atomicOr(err, ERR_TIMEOUT_MMA);  // and it does not count
+          const bool done = whole_part && atomicAdd(&ca.arrived[g.f0], 1) == g.parts - 1;
           if (done) ca.arrived[g.f0] = 0;
           sm.merge = done;
           __threadfence();
           mbar_arrive(&sm.merge_full);
         }
         __syncwarp();
-        if (!mbar_wait_short(&sm.merge_full, n_merge & 1)) ok = false;
+        if (!mbar_wait_warp(&sm.merge_full, n_merge & 1)) ok = false;
         ++n_merge;
         if (*reinterpret_cast<volatile int*>(&sm.merge) && real && ok) {
           // the first block's partial is of kind 1, the others' of kind 0

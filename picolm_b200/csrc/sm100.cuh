@@ -99,13 +99,27 @@ __device__ __forceinline__ bool mbar_sleep_wait(uint64_t* bar, uint32_t parity) 
       : "memory");
   return ok != 0;
 }
-__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_wait_short(uint64_t* bar, uint32_t parity,
+                                                uint64_t at_least_ns = 0) {
   if (mbar_sleep_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer(), lim = wait_limit_ns();
+  const uint64_t t0 = globaltimer(), set = wait_limit_ns();
+  const uint64_t lim = set > at_least_ns ? set : at_least_ns;
 #pragma unroll 1
   while (!mbar_sleep_wait(bar, parity))
     if (globaltimer() - t0 > lim) return false;
   return true;
+}
+
+// By a whole warp, with one verdict for all its lanes (which may read the clock
+// on different sides of the limit): what comes next may need the whole warp.
+__device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait_short(bar, parity));
+}
+
+// For a thread's own copies or MMAs in flight, before it leaves: however short
+// the limit is, they must not land in a block that is gone.
+__device__ __forceinline__ void mbar_wait_drained(uint64_t* bar, uint32_t parity) {
+  mbar_wait_short(bar, parity, kDefaultWaitLimitNs);
 }
 
 // ---------------------------------------------------------------- fences

@@ -742,6 +742,38 @@ def test_status_on_a_stream_that_waits_for_no_other():
     torch.cuda.synchronize()
 
 
+def test_waits_that_run_out_are_reported():
+    """A block's scheduler stays four segments ahead of the others, and waits
+    for a segment to end before it names a fifth: here, with seven segments
+    of 1024 tiles a block, for 0.28 ms at least (a tile's 8192 exponentials at
+    16 a clock take 0.27 us).  With a limit of 0.1 ms, after which a wait ends
+    within 0.04 ms, that runs out: the call says PL_ETIMEOUT, and the next one,
+    with the limit back, is right again."""
+    gen = generator(33)
+    c = Cache(16, 2, 64, n_pages=1024, n_seqs=1, max_pages=1024)
+    c.fill([0], [65536], gen)
+    n = 512
+    q = randn(gen, 2 * n, 1024)
+    seqs, counts = [0] * n, [2] * n
+    want = c.attend(seqs, counts, q, torch.empty_like(q), pb.PL_F32)
+    for t in (0, 2 * n - 2):
+        exact, most, vmax = c.reference([0], [2], q[t:t + 2])
+        assert bool(((want[t:t + 2].double() - exact).abs() <=
+                     attention_bound(pb.PL_F32, 64, 65536, most, vmax, exact)).all())
+    a, st = i32(seqs), i32(starts(counts))
+    with pb.Attn(1, 8, 2, 64) as at:
+        for _ in range(2):
+            at.set_wait_limit(1e-4)
+            out = torch.empty_like(q)
+            c.c.attend_dev(0, n, a.data_ptr(), st.data_ptr(), 2 * n, 2, pb.PL_F32, q.data_ptr(), 1024,
+                           out.data_ptr(), 1024, stream())
+            rc = c.c.status(stream())
+            at.set_wait_limit(2.0)
+            assert rc == pb.PL_ETIMEOUT
+            assert c.c.status(stream()) == pb.PL_OK
+            assert torch.equal(c.attend(seqs, counts, q, out, pb.PL_F32), want)
+
+
 def test_two_caches_on_two_streams():
     """Caches are independent: their calls may overlap."""
     gen = generator(23)
