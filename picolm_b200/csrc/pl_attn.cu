@@ -776,7 +776,10 @@ int finish_host_call(const uint32_t* h_err) {
 void free_ctx(Ctx* c) {
   if (!c) return;
   if (c->device >= 0) cudaSetDevice(c->device);
-  if (c->stream) cudaStreamSynchronize(c->stream);
+  if (c->stream) {
+    cudaStreamSynchronize(c->stream);
+    pl_module::kv8_wait_limit(pl::kDefaultWaitLimitNs);  // caches outlive the context
+  }
   cudaFree(c->d_k);
   cudaFree(c->d_v);
   cudaFree(c->d_cos);

@@ -774,6 +774,17 @@ def test_waits_that_run_out_are_reported():
             assert torch.equal(c.attend(seqs, counts, q, out, pb.PL_F32), want)
 
 
+def test_wait_limit_ends_with_its_context():
+    """The call of the test above, after a context that had set 0.1 ms."""
+    gen = generator(34)
+    c = Cache(16, 2, 64, n_pages=1024, n_seqs=1, max_pages=1024)
+    c.fill([0], [65536], gen)
+    q = randn(gen, 1024, 1024)
+    with pb.Attn(1, 8, 2, 64) as at:
+        at.set_wait_limit(1e-4)
+    c.attend([0] * 512, [2] * 512, q, torch.empty_like(q), pb.PL_F32)  # checks the status
+
+
 def test_two_caches_on_two_streams():
     """Caches are independent: their calls may overlap."""
     gen = generator(23)
