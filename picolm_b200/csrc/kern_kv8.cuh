@@ -181,7 +181,7 @@ __device__ __forceinline__ void rotate_pair8(int e, const pl_rope& r, const floa
 
 // x / by, correctly rounded, from the rounded reciprocal inv of by
 // (Markstein, 1990: one correction by the exact remainder gives the rounded
-// quotient), where nothing comes near the ends of the range.
+// quotient), where nothing comes near the ends of the range.  0 for -0.
 __device__ __forceinline__ float quotient(float x, float by, float inv) {
   const float q = __fmul_rn(x, inv);
   return fmaf(fmaf(-q, by, x), inv, q);
@@ -347,7 +347,7 @@ __global__ void __launch_bounds__(kAppendThreads, 3) kv8_append_kernel(
       for (int p = 0; p < kPasses; ++p)
 #pragma unroll 1
         for (int j = 0; j < 8; ++j) {
-          const float q = __fdiv_rn(x[p][0], by);  // in turn, to keep the code short
+          const float q = __fdiv_rn(x[p][0], by) + 0.f;  // in turn, to keep the code short
 #pragma unroll
           for (int m = 0; m < 7; ++m) x[p][m] = x[p][m + 1];
           x[p][7] = q;

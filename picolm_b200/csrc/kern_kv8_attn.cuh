@@ -364,7 +364,8 @@ __device__ __forceinline__ void append_row(const float (&x)[HD / 32], int lane, 
   }
   uint32_t code = 0;
 #pragma unroll
-  for (int j = 0; j < E; ++j) code |= encode1<FMT>(__fdiv_rn(x[j], by)) << (8 * j);
+  for (int j = 0; j < E; ++j)  // (+ 0: as quotient() has it, -0 becomes 0)
+    code |= encode1<FMT>(__fdiv_rn(x[j], by) + 0.f) << (8 * j);
   if (!(s < INFINITY)) code = 0;  // no code stands for a NaN
   const int el = lane * E;
   const uint32_t at = tile + tile_off<HD>(r, el >> 4) + (el & 15);

@@ -326,6 +326,56 @@ def test_same_call_twice_gives_the_same_bits():
         assert torch.equal(a, b)
 
 
+ROTATIONS = [dict(rope_dim=0), dict(rope_dim=10), dict(rope_dim=36), dict(rope_dim=48, base=500000.0), dict(),
+             dict(rope_dim=32, scaling=pb.PL_ROPE_SCALE_YARN, factor=16.0, orig_len=64, low=1.0, high=32.0)]
+
+
+@pytest.mark.parametrize("rotation", ROTATIONS, ids=["none", "10", "36", "48", "whole", "yarn32"])
+@pytest.mark.parametrize("layout", [pb.PL_ROPE_LLAMA, pb.PL_ROPE_QWEN])
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_decode_appends_as_append_does(head_dim, fmt, layout, rotation):
+    """The decode step stores the codes and scales of pl_kv8_append_dev, at the
+    start of a block, inside one and at its end, for rows that raise the
+    scale, that do not, that are 0 and that are not finite; and attends them."""
+    gen = generator(37)
+    lens = [0, 1, 5, 14, 15, 16, 31, 63, 64, 100, 127, 9, 40, 70]  # before the step
+    n, kd = len(lens), 4 * head_dim
+    seqs = [int(i) for i in torch.randperm(n, generator=torch.Generator().manual_seed(2))]
+    caches = [Cache(8, 4, head_dim, fmt, n_pages=48, n_seqs=n, max_pages=3, layout=layout, **rotation)
+              for _ in range(2)]
+    a, b = caches
+    b.codes.copy_(a.codes)
+    for c in caches:
+        c.resize(seqs, lens)
+    k, v = randn(gen, sum(lens), kd), randn(gen, sum(lens), kd)
+    for c in caches:
+        c.append(seqs, lens, k, v, pb.PL_F32)
+    saved = [(c.codes.clone(), c.scales.clone()) for c in caches]
+    assert torch.equal(a.codes, b.codes) and torch.equal(a.scales.view(torch.int32), b.scales.view(torch.int32))
+    for c in caches:
+        c.resize(seqs, [m + 1 for m in lens])
+    for dtype in DTYPES:
+        q, k, v = (randn(gen, n, w, dtype=TORCH[dtype]) for w in (2 * kd, kd, kd))
+        k[1::3] *= 20          # raise the scales
+        v[2::3] *= 20
+        k[4], v[5] = 0, 0
+        k[6, 3], k[7, kd - 1], v[8, head_dim], v[12, 5] = math.nan, math.inf, -math.inf, math.nan
+        for c, (codes, scales) in zip(caches, saved):
+            c.codes.copy_(codes)
+            c.scales.copy_(scales)
+        out = a.decode(seqs, q, k, v, torch.empty_like(q), dtype)
+        b.append(seqs, [1] * n, k, v, dtype)
+        assert torch.equal(a.codes, b.codes)
+        assert torch.equal(a.scales.isnan(), b.scales.isnan())
+        assert torch.equal(a.scales.nan_to_num(-1), b.scales.nan_to_num(-1))
+        fine = [i for i in range(n) if i not in (6, 7, 8, 12)]
+        t = torch.tensor(fine, device="cuda")
+        want, most, vmax = a.reference([seqs[i] for i in fine], [1] * len(fine), q[t])
+        assert bool(((out[t].double() - want).abs() <= attention_bound(dtype, head_dim, 128, most, vmax, want)).all())
+        assert torch.equal(b.attend(seqs, [1] * n, q, torch.empty_like(q), dtype)[t], out[t])
+
+
 # ------------------------------------------------------------------- pages
 class Books:
     """The page operations in plain Python."""
