@@ -314,6 +314,26 @@ def test_long_contexts_are_split(seqs, length):
             attend_and_check(c, list(range(seqs)), [count] * seqs, dtype, gen)
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize("rise", [1, -1], ids=["rising", "falling"])
+def test_outputs_leave_the_accumulator_several_times(fmt, head_dim, rise):
+    """24 items of 188 tiles: on up to 160 SMs a block has at least 29 of
+    their places, so most segments move O to its sums, every 4 tiles at
+    head_dim 64 and every 8 at 128, three times or more.  Scores and V scales
+    rise (or fall) all along, so the sums are rescaled as they are joined (or
+    carry the output)."""
+    gen = generator(35)
+    c = Cache(16, 8, head_dim, fmt, n_pages=188, n_seqs=1, max_pages=188)
+    c.fill([0], [12000], gen)
+    pages = c.table[0].long()
+    ramp = torch.linspace(-1, 1, 188 * 4, device="cuda").view(188, 1, 4) * rise
+    c.scales[pages, 0, :, 0] *= 2.0 ** (2 * ramp)      # scores of +-0.25 to +-4 standard deviations
+    c.scales[pages, 0, :, 1] *= 10.0 ** (4.5 * ramp - 1)  # values from 10^-5.5 to 10^3.5
+    for dtype in (pb.PL_F32, pb.PL_F16):
+        attend_and_check(c, [0], [300], dtype, gen)
+
+
 def test_same_call_twice_gives_the_same_bits():
     gen = generator(11)
     c = Cache(32, 4, 64, n_pages=200, n_seqs=6, max_pages=64)
@@ -328,6 +348,18 @@ def test_same_call_twice_gives_the_same_bits():
 
 ROTATIONS = [dict(rope_dim=0), dict(rope_dim=10), dict(rope_dim=36), dict(rope_dim=48, base=500000.0), dict(),
              dict(rope_dim=32, scaling=pb.PL_ROPE_SCALE_YARN, factor=16.0, orig_len=64, low=1.0, high=32.0)]
+
+
+@pytest.mark.parametrize("rotation", ROTATIONS, ids=["none", "10", "36", "48", "whole", "yarn32"])
+@pytest.mark.parametrize("layout", [pb.PL_ROPE_LLAMA, pb.PL_ROPE_QWEN])
+@pytest.mark.parametrize("head_dim", [64, 128])
+def test_attention_with_part_of_a_head_rotated(head_dim, layout, rotation):
+    gen = generator(36)
+    c = Cache(12, 4, head_dim, n_pages=32, n_seqs=3, max_pages=8, layout=layout, **rotation)
+    c.fill([0, 1, 2], [300, 77, 512], gen)
+    for dtype in DTYPES:
+        attend_and_check(c, [2, 0, 1], [1, 1, 1], dtype, gen)
+        attend_and_check(c, [2, 0, 1], [70, 3, 77], dtype, gen)
 
 
 @pytest.mark.parametrize("rotation", ROTATIONS, ids=["none", "10", "36", "48", "whole", "yarn32"])
