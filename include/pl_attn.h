@@ -466,8 +466,9 @@ int  pl_rope_rows_dev(const pl_rope *r, int dtype, int n, const int *d_pos,
  * several times.  The bound on device-side waits is pl_attn_set_wait_limit's
  * (2 s without a context); where several tokens attend, one wait may last as
  * long as a block's share of the rows (about 1 us for 64 of them), and a
- * call whose waits run out leaves its output undefined.  A call has n <= 1024 entries, and fewer than
- * 2^29 / (max_pages * n_kv_heads) (PL_EARG).
+ * call whose waits run out leaves its output undefined.  A call has n <= 1024
+ * entries, and one on rows fewer than 2^29 / (max_pages * n_kv_heads)
+ * (PL_EARG).
  * Inputs and outputs are `dtype` rows of heads x head_dim elements, 16-byte
  * aligned with strides (in elements) that are multiples of 16 bytes. */
 /* Bytes of the workspace of a cache of this shape. */
@@ -519,7 +520,13 @@ int  pl_kv8_append_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
 /* Causal attention: rows d_start[i] .. d_start[i+1]-1 of q are the last
  * positions of slot d_seqs[i] (d_start NULL: one each), rotated here; token
  * j of n_tok attends rows [0, len - n_tok + j].  A token with no row to
- * attend gets zeros; rows of d_out past d_start[n] are left as they are. */
+ * attend gets zeros; rows of d_out past d_start[n] are left as they are.
+ * Scores, softmax and sums are FP32.  BF16 queries are rounded to FP16 once
+ * after their rotation, relative to the row's largest element, and so are the
+ * softmax weights, where max_tok is above 1: 2^-11 relative, an eighth of
+ * what rounding the output costs.  FP32 and FP16 ones are carried in two FP16
+ * parts, 2^-22.  Sums of values times weights must stay inside FP32's range:
+ * |v| * rows below 3e38. */
 int  pl_kv8_attend_dev(const pl_kv8 *c, int layer, int n, const int *d_seqs,
                        const int *d_start, int total, int max_tok, int dtype,
                        const void *d_q, long long q_stride, void *d_out,

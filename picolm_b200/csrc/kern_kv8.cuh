@@ -198,9 +198,13 @@ __device__ __forceinline__ float quotient(float x, float by, float inv) {
 // e4m3 has a code for NaN, and attention multiplies the codes of rows that a
 // mask hides by a weight of 0, which a NaN would survive.
 //
-// Cosines are FP64 and rounded once, so that codes do not depend on how a
-// row was appended; a block of rows takes two sincospi a pair (its first
-// row's and one row's step) and turns from row to row by FP64 products.
+// Cosines are FP64 and rounded once; a block of rows takes a sincospi or two a
+// pair (its first row's and one row's step) and turns from row to row by FP64
+// products.  A call of one token takes a sincospi of the row itself, as the
+// decode step does; the two are apart by up to (position + 32) 2^-52 (for
+// frequencies up to 1), so how rows were appended can move a cosine by one
+// rounding to FP32 where it lies that near to a border.  And rows that came one
+// by one have been rounded again each time the scale of their block grew.
 //
 // Should be bound by HBM, is bound by instructions and the latency of few
 // warps (51% of the issue slots, at 18 warps an SM): 8

@@ -60,10 +60,10 @@ constexpr int kKv8MaxGroup = 8;  // query heads per KV head
 //
 // On one B200: 64 sequences of 2048 rows, 32/4 heads of 64, FP32: 26 us (69
 // MB); 32 ragged ones up to 8192 rows, 32/8 heads of 128, BF16: 85 us (335
-// MB, 3.9 TB/s); one of 32768, 32/8 of 64: 20 us; one of 256 rows: 10 us.  Of
-// the 26 us about 11 stream the tiles, at 5.9 TB/s; before that a block reads
-// and scans the books (1.3), finds its first tile (2.5) and rotates q (0.8),
-// and after it the runs that cross blocks are merged (5).  At head_dim 128
+// MB, 3.9 TB/s); one of 32768, 32/8 of 64: 19 us; one of 256 rows: 10 us.
+// Streaming takes 11 of the 26 us at a copy's rate; before it a block reads
+// and scans the books, finds its first tile and rotates q, and after it the
+// runs that cross blocks are merged.  At head_dim 128
 // the stream runs at the pace of its eight warps, which have 255 registers
 // each; more warps spill and are slower, as were four of 64-row tiles.
 //
@@ -468,7 +468,8 @@ __global__ void __launch_bounds__(DecShape<HD>::kThreads, 1) kv8_decode_kernel(
     __syncthreads();
   }
   const int total = sm.prefix[a.n];
-  // at least a tile for each warp of a block: fewer blocks share a run then
+  // about a tile for each warp (9 tiles make two blocks of 4 and 5): fewer
+  // blocks share a run then
   const DecWork<HD> work{sm.prefix, a.n, heads, total,
                          min(static_cast<int>(gridDim.x), (total + W - 1) / W)};
   const int blk = blockIdx.x;

@@ -25,7 +25,7 @@
 //   warps 8-11       converters: codes to FP16 -- every code is exact -- in
 //                    swizzled K and V tiles
 //   warps 12, 13     MMA issuers of slots A, B (12 allocates TMEM)
-//   warp 14          scheduler: publishes the slice's segments, two ahead
+//   warp 14          scheduler: publishes the slice's segments, up to four ahead
 //   warp 15          loader: bulk copies of codes and scales from the pages
 //                    into a ring, tiles ahead of the converters
 // Per tile n the issuer of slot x issues S(n) = Q K^T and then O += P(n-1) V,
@@ -39,7 +39,7 @@
 // Measured on one B200: a prompt of 2048 FP32 tokens, 32/4 heads of 64: 92 us
 // (17 GFLOP, 187 TFLOP/s; the tensor pipe, which does it twice, is active
 // 18% of the time, issue slots 45%); 4 chunks of up to 1024 BF16 tokens
-// behind up to 8192 rows, 32/8 heads of 128: 461 us (682 TFLOP/s, 32%, 50%).
+// behind up to 8192 rows, 32/8 heads of 128: 460 us (684 TFLOP/s, 32%, 50%).
 // A pair of tiles takes 1.5 to 1.8 us, of which 2^x alone would take 0.55;
 // the start and the end of an item another 7 to 9 pairs' time.
 //
@@ -117,7 +117,8 @@ struct ChShape {
   static_assert(2 * kBN + 2 * HD + 2 * kPCols + (kSumsInTmem && PARTS == 2 ? 2 * HD : 0) <= 512,
                 "TMEM columns");
   // Places of the list before an item's tiles: what its start (rows of q) and
-  // end (O, a merge) take, in tiles; more where the rows are longer.  1 x 2048
+  // end (O, a merge) take, in tiles; more where the rows are longer.  Measured
+  // in the types named, used for all.  1 x 2048
   // tokens / 4 x 1024 behind 8192 rows / 16 x 64 behind 1024, in us, at
   // head_dim 64 in FP32: 106, 518, 59 with 3; 98, 502, 55 with 7; 104, 502,
   // 53 with 12.  At head_dim 128 in BF16: 121, 477, 70 with 3; 107, 465, 61
@@ -764,7 +765,10 @@ __global__ void __launch_bounds__(kChThreads, 1) kv8_chunk_kernel(
       };
       for (int j = 0; j < nt && active; ++j, ++A) {
         const int n = J + j;
-        // (the scales are the converters' writes: their barriers too)
+        // (the scales are the converters' writes: their barriers too.  A slot
+        // that sat out eight tiles or more can find the barrier two phases back
+        // and pass early; s_full then orders the writes, since the issuer took
+        // the same warps' k_full of this tile, arrived at after the scales.)
         ok = __all_sync(0xffffffffu, ok && mbar_wait_short(&sm.scale_full[n & 7], (n >> 3) & 1) &&
                                          mbar_wait_short(&sm.s_full[x], A & 1));
         if (!ok) continue;

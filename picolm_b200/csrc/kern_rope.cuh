@@ -9,7 +9,8 @@
 // respect to x) is the same with -s.  There is no table of positions: the
 // angle is taken in FP64, so a position may be any non-negative int.
 //
-// Bound by HBM: each element is read and written once.  A block rotates all
+// Should be bound by HBM, as each element is read and written once; is bound by
+// the start of its blocks.  A block rotates all
 // heads of a few rows, so that the FP64 cosines (about a hundred instructions
 // each) are computed once per (row, pair) into shared memory and not once
 // per head.  8192 rows of 32 + 8 heads of 128 in BF16, half of each rotated
